@@ -1,0 +1,659 @@
+// C-ABI of the serving operators: see include/ft_serving.h.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <new>
+#include <vector>
+
+#include "serving_kernels.h"
+
+using namespace ftg;
+
+namespace ftg {
+int noalloc_fail(int code, const char* fmt, ...);  // sets the thread's last-error text (api.cu)
+}
+
+namespace {
+
+#define SERVE_CUDA(call)                                                                                     \
+  do {                                                                                                       \
+    cudaError_t err_ = (call);                                                                               \
+    if (err_ != cudaSuccess) return noalloc_fail(FT_ERR_CUDA, "%s failed: %s", #call, cudaGetErrorString(err_)); \
+  } while (0)
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// The rules every ft_rows has to meet; `heads` is what the operator expects there.
+int check_rows(const ft_rows* r, const char* name, int heads) {
+  if (r == nullptr || r->data == nullptr) return noalloc_fail(FT_ERR_INVALID, "null %s", name);
+  if (r->heads != heads) return noalloc_fail(FT_ERR_INVALID, "%s has %d heads where %d are expected", name, r->heads, heads);
+  if (!aligned16(r->data) || r->token_stride % 8 != 0 || r->head_stride % 8 != 0 || r->token_stride < 0 || r->head_stride < 0) {
+    return noalloc_fail(FT_ERR_INVALID, "%s must be 16-byte aligned with strides that are multiples of 8 elements", name);
+  }
+  return FT_OK;
+}
+
+// The tensor-copy engine steps through rows that do not overlap: a broadcast head or token is refused.
+int check_apart(const ft_rows* r, const char* name, int tokens, int head_dim) {
+  if ((r->heads > 1 && r->head_stride < head_dim) || (tokens > 1 && r->token_stride < head_dim)) {
+    return noalloc_fail(FT_ERR_INVALID, "the heads and tokens of %s must not share memory (strides %lld, %lld)", name, r->token_stride, r->head_stride);
+  }
+  return FT_OK;
+}
+
+int check_dtype(int dtype) {
+  if (dtype != FT_SRC_BF16 && dtype != FT_SRC_F16) return noalloc_fail(FT_ERR_INVALID, "dtype must be FT_SRC_BF16 or FT_SRC_F16");
+  return FT_OK;
+}
+
+Rows to_rows(const ft_rows* r) { return Rows{static_cast<uint16_t*>(r->data), r->token_stride, r->head_stride}; }
+
+int check_cache(const ft_kv_cache* c) {
+  if (c == nullptr || c->k == nullptr || c->v == nullptr) return noalloc_fail(FT_ERR_INVALID, "null cache, K or V");
+  const int rc = check_dtype(c->dtype);
+  if (rc != FT_OK) return rc;
+  if (c->layers <= 0 || c->layers > 32767 || c->pages <= 0 || c->kv_heads <= 0 || (c->head_dim != 64 && c->head_dim != 128)) {
+    return noalloc_fail(FT_ERR_INVALID, "the cache needs 1 to 32767 layers, pages, key heads and head_dim 64 or 128 (got %d, %d, %d, %d)", c->layers,
+                        c->pages, c->kv_heads, c->head_dim);
+  }
+  if (c->page_size < 8 || c->page_size > 256 || (c->page_size & (c->page_size - 1)) != 0) {
+    return noalloc_fail(FT_ERR_INVALID, "page_size must be a power of two from 8 to 256 (got %d)", c->page_size);
+  }
+  const long long d = c->head_dim;
+  const bool by_token = c->token_stride == c->kv_heads * d && c->head_stride == d;
+  const bool by_head = c->token_stride == d && c->head_stride == c->page_size * d;
+  if (!by_token && !by_head && !(c->kv_heads == 1 && c->token_stride == d)) {
+    return noalloc_fail(FT_ERR_INVALID, "a page must be dense, by token (strides %lld, %lld) or by head (%lld, %lld)", c->kv_heads * d, d, d,
+                        c->page_size * d);
+  }
+  if (!aligned16(c->k) || !aligned16(c->v) || c->page_stride % 8 != 0 || c->layer_stride % 8 != 0 || c->page_stride < c->page_size * c->kv_heads * d ||
+      c->layer_stride < 0) {
+    return noalloc_fail(FT_ERR_INVALID, "K and V must be 16-byte aligned, with page and layer strides that are multiples of 8 elements, and pages must not overlap");
+  }
+  return FT_OK;
+}
+
+int check_scale(float scale) {
+  if (!(scale >= 0.0f) || !std::isfinite(scale)) return noalloc_fail(FT_ERR_INVALID, "scale must be positive and finite (0: 1 / sqrt(head_dim))");
+  return FT_OK;
+}
+
+int check_device() {
+  int device = 0, major = 0;
+  SERVE_CUDA(cudaGetDevice(&device));
+  SERVE_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
+  if (major != 10) return noalloc_fail(FT_ERR_UNSUPPORTED, "this library needs an sm_100 GPU (found compute capability %d)", major);
+  return FT_OK;
+}
+
+}  // namespace
+
+struct ft_rotary_handle {
+  ft_rotary_options options{};
+  double* turns = nullptr;  // device: frequencies in turns per position
+};
+
+struct ft_page_pool {
+  int page_size = 0;
+  std::vector<int> users;      // per page: sequences that hold it
+  std::vector<int> free_list;  // a heap, lowest page on top
+  struct Sequence {
+    bool used = false;
+    int length = 0;
+    std::vector<int> pages;
+  };
+  std::vector<Sequence> sequences;
+
+  Sequence* find(int id) { return id >= 0 && id < static_cast<int>(sequences.size()) && sequences[id].used ? &sequences[id] : nullptr; }
+  int take() {
+    std::pop_heap(free_list.begin(), free_list.end(), std::greater<int>());
+    const int page = free_list.back();
+    free_list.pop_back();
+    users[page] = 1;
+    return page;
+  }
+  void drop(int page) {
+    if (--users[page] == 0) {
+      free_list.push_back(page);  // capacity for every page is reserved at creation
+      std::push_heap(free_list.begin(), free_list.end(), std::greater<int>());
+    }
+  }
+};
+
+extern "C" {
+
+// ---- rotary positions -----------------------------------------------------------
+
+void ft_rotary_options_default(ft_rotary_options* o, int head_dim) {
+  if (o == nullptr) return;
+  std::memset(o, 0, sizeof(*o));
+  o->head_dim = head_dim;
+  o->rotary_dim = head_dim;
+  o->scaling = FT_ROTARY_PLAIN;
+  o->base = 10000.0;
+  o->factor = 1.0;
+  o->low = 1.0;
+  o->high = 4.0;
+  o->magnitude = 1.0;
+}
+
+int ft_rotary_frequencies(const ft_rotary_options* o, double* out) {
+  if (o == nullptr || out == nullptr) return noalloc_fail(FT_ERR_INVALID, "null options or output pointer");
+  if (o->head_dim <= 0 || o->head_dim > 256 || o->head_dim % 16 != 0 || o->rotary_dim <= 0 || o->rotary_dim > o->head_dim || o->rotary_dim % 16 != 0) {
+    return noalloc_fail(FT_ERR_INVALID, "head_dim (at most 256) and rotary_dim (at most head_dim) must be positive multiples of 16 (got %d, %d)",
+                        o->head_dim, o->rotary_dim);
+  }
+  if (!(o->base > 0.0) || !std::isfinite(o->base) || !(o->factor > 0.0) || !std::isfinite(o->factor) || !std::isfinite(o->magnitude)) {
+    return noalloc_fail(FT_ERR_INVALID, "base and factor must be positive, magnitude finite");
+  }
+  if (o->scaling < FT_ROTARY_PLAIN || o->scaling > FT_ROTARY_BY_PARTS) return noalloc_fail(FT_ERR_INVALID, "unknown scaling %d", o->scaling);
+  if (o->scaling == FT_ROTARY_BY_PARTS &&
+      (!(o->original_length > 0.0) || !std::isfinite(o->original_length) || !(o->high > o->low) || !std::isfinite(o->low) || !std::isfinite(o->high))) {
+    return noalloc_fail(FT_ERR_INVALID, "scaling by parts needs original_length > 0 and high > low");
+  }
+  const double two_pi = 6.283185307179586476925286766559;
+  const double dim = o->rotary_dim;
+  const double base = o->scaling == FT_ROTARY_BASE ? o->base * std::pow(o->factor, dim / (dim - 2.0)) : o->base;
+  for (int i = 0; i < o->rotary_dim / 2; ++i) {
+    double f = std::pow(base, -2.0 * i / dim);
+    if (o->scaling == FT_ROTARY_LINEAR) f /= o->factor;
+    if (o->scaling == FT_ROTARY_BY_PARTS) {
+      const double keep = std::min(1.0, std::max(0.0, (o->original_length * f / two_pi - o->low) / (o->high - o->low)));
+      f *= keep + (1.0 - keep) / o->factor;
+    }
+    out[i] = f;
+  }
+  return FT_OK;
+}
+
+int ft_rotary_destroy(ft_rotary_handle* h) {
+  if (h == nullptr) return FT_OK;
+  cudaFree(h->turns);
+  delete h;
+  return FT_OK;
+}
+
+int ft_rotary_prepare(ft_rotary_handle** handle, const ft_rotary_options* options, void* stream) {
+  if (handle == nullptr) return noalloc_fail(FT_ERR_INVALID, "null handle pointer");
+  *handle = nullptr;
+  double turns[128];
+  int rc = ft_rotary_frequencies(options, turns);
+  if (rc == FT_OK) rc = check_device();
+  if (rc != FT_OK) return rc;
+  const int count = options->rotary_dim / 2;
+  for (int i = 0; i < count; ++i) turns[i] /= 6.283185307179586476925286766559;
+  ft_rotary_handle* h = new (std::nothrow) ft_rotary_handle();
+  if (h == nullptr) return noalloc_fail(FT_ERR_INVALID, "out of host memory");
+  h->options = *options;
+  cudaError_t err = cudaMalloc(reinterpret_cast<void**>(&h->turns), count * sizeof(double));
+  // pageable host memory: the copy has left `turns` when the call returns; the wait makes the handle valid on every stream
+  if (err == cudaSuccess) err = cudaMemcpyAsync(h->turns, turns, count * sizeof(double), cudaMemcpyHostToDevice, static_cast<cudaStream_t>(stream));
+  if (err == cudaSuccess) err = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
+  if (err != cudaSuccess) {
+    ft_rotary_destroy(h);
+    return noalloc_fail(FT_ERR_CUDA, "preparing the rotary frequencies failed: %s", cudaGetErrorString(err));
+  }
+  *handle = h;
+  return FT_OK;
+}
+
+static void use_rotary(RotaryParams* p, const ft_rotary_handle* h) {
+  p->turns = h->turns;
+  p->rotary_dim = h->options.rotary_dim;
+  p->head_dim = h->options.head_dim;
+  p->interleaved = h->options.interleaved != 0;
+  p->magnitude = static_cast<float>(h->options.magnitude);
+}
+
+int ft_rotary_run(const ft_rotary_handle* h, const ft_rows* q, const ft_rows* q_out, const ft_rows* k, const ft_rows* k_out, const long long* positions,
+                  int tokens, int dtype, int inverse, void* stream) {
+  if (h == nullptr || positions == nullptr) return noalloc_fail(FT_ERR_INVALID, "null handle or positions");
+  if (tokens < 0) return noalloc_fail(FT_ERR_INVALID, "negative token count");
+  if (q == nullptr || q->heads <= 0 || (k != nullptr && k->heads <= 0)) return noalloc_fail(FT_ERR_INVALID, "q needs at least one head, and k if given");
+  int rc = check_dtype(dtype);
+  if (rc == FT_OK) rc = check_rows(q, "q", q->heads);
+  if (rc == FT_OK) rc = check_rows(q_out, "q_out", q->heads);
+  if (rc == FT_OK && k != nullptr) rc = check_rows(k, "k", k->heads);
+  if (rc == FT_OK && k != nullptr) rc = check_rows(k_out, "k_out", k->heads);
+  if (rc != FT_OK) return rc;
+  RotaryParams p{};
+  use_rotary(&p, h);
+  p.q = to_rows(q);
+  p.q_out = to_rows(q_out);
+  p.q_heads = q->heads;
+  if (k != nullptr) {
+    p.k = to_rows(k);
+    p.k_out = to_rows(k_out);
+    p.k_heads = k->heads;
+  }
+  p.positions = positions;
+  p.tokens = tokens;
+  p.inverse = inverse != 0;
+  SERVE_CUDA(launch_rotary(p, dtype, static_cast<cudaStream_t>(stream)));
+  return FT_OK;
+}
+
+// ---- paged key/value cache -------------------------------------------------------
+
+int ft_kv_cache_append(const ft_kv_cache* cache, int layer, const ft_rows* k, const ft_rows* v, const long long* slots, int tokens,
+                       const ft_rotary_handle* rotary, const long long* positions, const ft_rows* q, const ft_rows* q_out, void* stream) {
+  int rc = check_cache(cache);
+  if (rc != FT_OK) return rc;
+  if (layer < 0 || layer >= cache->layers) return noalloc_fail(FT_ERR_INVALID, "layer %d is outside the cache's %d", layer, cache->layers);
+  if (slots == nullptr) return noalloc_fail(FT_ERR_INVALID, "null slots");
+  if (tokens < 0) return noalloc_fail(FT_ERR_INVALID, "negative token count");
+  rc = check_rows(k, "k", cache->kv_heads);
+  if (rc == FT_OK) rc = check_rows(v, "v", cache->kv_heads);
+  if (rc != FT_OK) return rc;
+  if (rotary == nullptr && q != nullptr) return noalloc_fail(FT_ERR_INVALID, "q is only rotated with a rotary handle");
+  if (rotary != nullptr && positions == nullptr) return noalloc_fail(FT_ERR_INVALID, "null positions");
+  if (rotary != nullptr && rotary->options.head_dim != cache->head_dim) {
+    return noalloc_fail(FT_ERR_INVALID, "the rotary handle is for head_dim %d, the cache has %d", rotary->options.head_dim, cache->head_dim);
+  }
+  RotaryParams p{};
+  p.head_dim = cache->head_dim;
+  if (rotary != nullptr) use_rotary(&p, rotary);
+  if (q != nullptr) {
+    if (q->heads <= 0) return noalloc_fail(FT_ERR_INVALID, "q needs at least one head");
+    rc = check_rows(q, "q", q->heads);
+    if (rc == FT_OK) rc = check_rows(q_out, "q_out", q->heads);
+    if (rc != FT_OK) return rc;
+    p.q = to_rows(q);
+    p.q_out = to_rows(q_out);
+    p.q_heads = q->heads;
+  }
+  p.k = to_rows(k);
+  p.v = to_rows(v);
+  p.k_heads = p.v_heads = cache->kv_heads;
+  p.positions = positions;
+  p.slots = slots;
+  p.k_cache = static_cast<uint16_t*>(cache->k) + layer * cache->layer_stride;
+  p.v_cache = static_cast<uint16_t*>(cache->v) + layer * cache->layer_stride;
+  p.page_stride = cache->page_stride;
+  p.cache_token_stride = cache->token_stride;
+  p.cache_head_stride = cache->head_stride;
+  p.page_size = cache->page_size;
+  p.slot_count = static_cast<long long>(cache->pages) * cache->page_size;
+  p.tokens = tokens;
+  SERVE_CUDA(launch_rotary(p, cache->dtype, static_cast<cudaStream_t>(stream)));
+  return FT_OK;
+}
+
+int ft_kv_cache_copy_pages(const ft_kv_cache* cache, const int* sources, const int* targets, int count, void* stream) {
+  int rc = check_cache(cache);
+  if (rc != FT_OK) return rc;
+  if (count < 0 || count > (1 << 24) || (count > 0 && (sources == nullptr || targets == nullptr))) {
+    return noalloc_fail(FT_ERR_INVALID, "copying pages needs 0 to 2^24 pairs with sources and targets (got %d)", count);
+  }
+  CopyPagesParams p{};
+  p.k = static_cast<uint16_t*>(cache->k);
+  p.v = static_cast<uint16_t*>(cache->v);
+  p.layer_stride = cache->layer_stride;
+  p.page_stride = cache->page_stride;
+  p.layers = cache->layers;
+  p.pages = cache->pages;
+  p.page_elements = cache->page_size * cache->kv_heads * cache->head_dim;
+  p.count = count;
+  p.sources = sources;
+  p.targets = targets;
+  SERVE_CUDA(launch_copy_pages(p, static_cast<cudaStream_t>(stream)));
+  return FT_OK;
+}
+
+int ft_kv_cache_accept(const ft_kv_cache* cache, const int* page_table, int table_pages, int table_stride, const int* lengths,
+                       const int* drafted_offsets, const int* accepted, const int* accepted_offsets, int batch, int* new_lengths, void* stream) {
+  int rc = check_cache(cache);
+  if (rc != FT_OK) return rc;
+  if (batch < 0 || table_pages <= 0 || table_stride < table_pages) {
+    return noalloc_fail(FT_ERR_INVALID, "batch must not be negative, the page table needs columns and a stride that holds them");
+  }
+  if (page_table == nullptr || lengths == nullptr || drafted_offsets == nullptr || accepted == nullptr || accepted_offsets == nullptr ||
+      new_lengths == nullptr) {
+    return noalloc_fail(FT_ERR_INVALID, "null page table, lengths, offsets or accepted tokens");
+  }
+  if (lengths == new_lengths) return noalloc_fail(FT_ERR_INVALID, "new_lengths must not be the lengths array");
+  AcceptParams p{};
+  p.k = static_cast<uint16_t*>(cache->k);
+  p.v = static_cast<uint16_t*>(cache->v);
+  p.layer_stride = cache->layer_stride;
+  p.page_stride = cache->page_stride;
+  p.token_stride = cache->token_stride;
+  p.head_stride = cache->head_stride;
+  p.layers = cache->layers;
+  p.pages = cache->pages;
+  p.page_size = cache->page_size;
+  p.kv_heads = cache->kv_heads;
+  p.head_dim = cache->head_dim;
+  p.page_table = page_table;
+  p.table_pages = table_pages;
+  p.table_stride = table_stride;
+  p.lengths = lengths;
+  p.drafted_offsets = drafted_offsets;
+  p.accepted = accepted;
+  p.accepted_offsets = accepted_offsets;
+  p.batch = batch;
+  p.new_lengths = new_lengths;
+  SERVE_CUDA(launch_accept(p, static_cast<cudaStream_t>(stream)));
+  return FT_OK;
+}
+
+// ---- page pool -------------------------------------------------------------------
+
+int ft_page_pool_create(ft_page_pool** pool, int pages, int page_size) {
+  if (pool == nullptr) return noalloc_fail(FT_ERR_INVALID, "null pool pointer");
+  *pool = nullptr;
+  if (pages <= 0 || page_size <= 0) return noalloc_fail(FT_ERR_INVALID, "a pool needs pages and a page size");
+  try {
+    ft_page_pool* p = new ft_page_pool();
+    *pool = p;
+    p->page_size = page_size;
+    p->users.assign(pages, 0);
+    p->free_list.resize(pages);
+    for (int i = 0; i < pages; ++i) p->free_list[i] = i;  // ascending: a heap already
+  } catch (const std::bad_alloc&) {
+    delete *pool;
+    *pool = nullptr;
+    return noalloc_fail(FT_ERR_INVALID, "out of host memory");
+  }
+  return FT_OK;
+}
+
+int ft_page_pool_destroy(ft_page_pool* pool) {
+  delete pool;
+  return FT_OK;
+}
+
+int ft_page_pool_free_pages(const ft_page_pool* pool) {
+  if (pool == nullptr) return noalloc_fail(FT_ERR_INVALID, "null pool");
+  return static_cast<int>(pool->free_list.size());
+}
+
+int ft_page_pool_new_sequence(ft_page_pool* pool, int* sequence) {
+  if (pool == nullptr || sequence == nullptr) return noalloc_fail(FT_ERR_INVALID, "null pool or sequence pointer");
+  auto& all = pool->sequences;
+  size_t id = 0;
+  while (id < all.size() && all[id].used) ++id;
+  try {
+    if (id == all.size()) all.emplace_back();
+  } catch (const std::bad_alloc&) {
+    return noalloc_fail(FT_ERR_INVALID, "out of host memory");
+  }
+  all[id].used = true;
+  all[id].length = 0;
+  all[id].pages.clear();
+  *sequence = static_cast<int>(id);
+  return FT_OK;
+}
+
+int ft_page_pool_fork(ft_page_pool* pool, int sequence, int* child) {
+  if (pool == nullptr || child == nullptr) return noalloc_fail(FT_ERR_INVALID, "null pool or sequence pointer");
+  if (pool->find(sequence) == nullptr) return noalloc_fail(FT_ERR_INVALID, "no sequence %d", sequence);
+  int id = 0;
+  const int rc = ft_page_pool_new_sequence(pool, &id);
+  if (rc != FT_OK) return rc;
+  ft_page_pool::Sequence& parent = pool->sequences[sequence];
+  ft_page_pool::Sequence& made = pool->sequences[id];
+  try {
+    made.pages = parent.pages;
+  } catch (const std::bad_alloc&) {
+    made.used = false;
+    return noalloc_fail(FT_ERR_INVALID, "out of host memory");
+  }
+  made.length = parent.length;
+  for (int page : made.pages) ++pool->users[page];
+  *child = id;
+  return FT_OK;
+}
+
+int ft_page_pool_free(ft_page_pool* pool, int sequence) {
+  if (pool == nullptr) return noalloc_fail(FT_ERR_INVALID, "null pool");
+  ft_page_pool::Sequence* s = pool->find(sequence);
+  if (s == nullptr) return noalloc_fail(FT_ERR_INVALID, "no sequence %d", sequence);
+  for (int page : s->pages) pool->drop(page);
+  s->pages.clear();
+  s->length = 0;
+  s->used = false;
+  return FT_OK;
+}
+
+int ft_page_pool_extend(ft_page_pool* pool, int sequence, int tokens, int* source, int* target) {
+  if (pool == nullptr || source == nullptr || target == nullptr) return noalloc_fail(FT_ERR_INVALID, "null pool or pair pointer");
+  *source = *target = -1;
+  ft_page_pool::Sequence* s = pool->find(sequence);
+  if (s == nullptr) return noalloc_fail(FT_ERR_INVALID, "no sequence %d", sequence);
+  if (tokens < 0 || tokens > INT32_MAX - s->length) return noalloc_fail(FT_ERR_INVALID, "a sequence cannot grow by %d tokens", tokens);
+  if (tokens == 0) return FT_OK;
+  const int size = pool->page_size, length = s->length + tokens;
+  const size_t held = s->pages.size(), need = (static_cast<size_t>(length) + size - 1) / size;
+  // the page that the first new token goes to is written: it must be this sequence's alone
+  const bool copy = s->length % size != 0 && pool->users[s->pages[s->length / size]] > 1;
+  const size_t take = need - held + (copy ? 1 : 0);
+  if (take > pool->free_list.size()) {
+    return noalloc_fail(FT_ERR_INVALID, "the pool has %zu free pages, %zu are needed", pool->free_list.size(), take);
+  }
+  try {
+    s->pages.reserve(need);
+  } catch (const std::bad_alloc&) {
+    return noalloc_fail(FT_ERR_INVALID, "out of host memory");
+  }
+  if (copy) {
+    int& last = s->pages[s->length / size];
+    *source = last;
+    *target = pool->take();
+    pool->drop(last);
+    last = *target;
+  }
+  while (s->pages.size() < need) s->pages.push_back(pool->take());
+  s->length = length;
+  return FT_OK;
+}
+
+int ft_page_pool_truncate(ft_page_pool* pool, int sequence, int length) {
+  if (pool == nullptr) return noalloc_fail(FT_ERR_INVALID, "null pool");
+  ft_page_pool::Sequence* s = pool->find(sequence);
+  if (s == nullptr) return noalloc_fail(FT_ERR_INVALID, "no sequence %d", sequence);
+  if (length < 0 || length > s->length) return noalloc_fail(FT_ERR_INVALID, "sequence %d holds %d tokens, it cannot be cut to %d", sequence, s->length, length);
+  const size_t need = (static_cast<size_t>(length) + pool->page_size - 1) / pool->page_size;
+  while (s->pages.size() > need) {
+    pool->drop(s->pages.back());
+    s->pages.pop_back();
+  }
+  s->length = length;
+  return FT_OK;
+}
+
+int ft_page_pool_length(const ft_page_pool* pool, int sequence) {
+  if (pool == nullptr) return noalloc_fail(FT_ERR_INVALID, "null pool");
+  const ft_page_pool::Sequence* s = const_cast<ft_page_pool*>(pool)->find(sequence);
+  if (s == nullptr) return noalloc_fail(FT_ERR_INVALID, "no sequence %d", sequence);
+  return s->length;
+}
+
+int ft_page_pool_pages(const ft_page_pool* pool, int sequence, int* out, int capacity) {
+  if (pool == nullptr || (out == nullptr && capacity > 0) || capacity < 0) return noalloc_fail(FT_ERR_INVALID, "null pool or page array");
+  const ft_page_pool::Sequence* s = const_cast<ft_page_pool*>(pool)->find(sequence);
+  if (s == nullptr) return noalloc_fail(FT_ERR_INVALID, "no sequence %d", sequence);
+  const int count = static_cast<int>(s->pages.size());
+  std::copy(s->pages.begin(), s->pages.begin() + std::min(count, capacity), out);
+  return count;
+}
+
+int ft_page_pool_compact(ft_page_pool* pool, int* sources, int* targets, int capacity, int* count) {
+  if (pool == nullptr || count == nullptr || capacity < 0 || (capacity > 0 && (sources == nullptr || targets == nullptr))) {
+    return noalloc_fail(FT_ERR_INVALID, "null pool, pairs or count");
+  }
+  *count = 0;
+  try {
+    std::vector<int> moved(pool->users.size(), -1);
+    std::vector<int> free_after;
+    free_after.reserve(pool->users.size());
+    int low = 0, high = static_cast<int>(pool->users.size()) - 1, n = 0;
+    while (n < capacity) {
+      while (low < high && pool->users[low] > 0) ++low;
+      while (low < high && pool->users[high] == 0) --high;
+      if (low >= high) break;
+      sources[n] = high;
+      targets[n++] = low;
+      moved[high] = low;
+      pool->users[low] = pool->users[high];
+      pool->users[high] = 0;
+    }
+    for (auto& s : pool->sequences) {
+      for (int& page : s.pages) {
+        if (moved[page] >= 0) page = moved[page];
+      }
+    }
+    pool->free_list.clear();
+    for (int i = 0; i < static_cast<int>(pool->users.size()); ++i) {
+      if (pool->users[i] == 0) pool->free_list.push_back(i);
+    }
+    *count = n;
+  } catch (const std::bad_alloc&) {
+    return noalloc_fail(FT_ERR_INVALID, "out of host memory");
+  }
+  return FT_OK;
+}
+
+// ---- attention -------------------------------------------------------------------
+
+size_t ft_attention_workspace(void) { return 16; }
+
+static int check_attention_call(const void* workspace, size_t workspace_bytes, const int* status, int group_heads, int kv_heads) {
+  if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < ft_attention_workspace()) {
+    return noalloc_fail(FT_ERR_INVALID, "the workspace must be 16-byte aligned and hold ft_attention_workspace() bytes (%zu given)", workspace_bytes);
+  }
+  if (status == nullptr) return noalloc_fail(FT_ERR_INVALID, "null status");
+  if (kv_heads <= 0 || group_heads <= 0 || group_heads % kv_heads != 0 || group_heads / kv_heads > 128) {
+    return noalloc_fail(FT_ERR_INVALID, "query heads (%d) must be 1 to 128 times the key heads (%d)", group_heads, kv_heads);
+  }
+  return FT_OK;
+}
+
+int ft_prompt_attention_run(const ft_prompt_attention_args* a, void* workspace, size_t workspace_bytes, int* status, void* stream) {
+  if (a == nullptr) return noalloc_fail(FT_ERR_INVALID, "null arguments");
+  int rc = check_attention_call(workspace, workspace_bytes, status, a->q.heads, a->k.heads);
+  if (rc == FT_OK) rc = check_dtype(a->dtype);
+  if (rc == FT_OK) rc = check_scale(a->scale);
+  if (rc != FT_OK) return rc;
+  if (a->head_dim != 64 && a->head_dim != 128) return noalloc_fail(FT_ERR_INVALID, "head_dim must be 64 or 128 (got %d)", a->head_dim);
+  if (a->batch < 0 || a->query_tokens < 0 || a->key_tokens < 0) return noalloc_fail(FT_ERR_INVALID, "negative batch or token count");
+  if (a->batch == 0 || a->query_tokens == 0) return FT_OK;
+  if (a->q_offsets == nullptr) return noalloc_fail(FT_ERR_INVALID, "null q_offsets");
+  rc = check_rows(&a->q, "q", a->q.heads);
+  if (rc == FT_OK) rc = check_rows(&a->out, "out", a->q.heads);
+  if (rc == FT_OK && a->key_tokens > 0) rc = check_rows(&a->k, "k", a->k.heads);
+  if (rc == FT_OK && a->key_tokens > 0) rc = check_rows(&a->v, "v", a->k.heads);
+  if (rc == FT_OK) rc = check_apart(&a->q, "q", a->query_tokens, a->head_dim);
+  if (rc == FT_OK) rc = check_apart(&a->out, "out", a->query_tokens, a->head_dim);
+  if (rc == FT_OK && a->key_tokens > 0) rc = check_apart(&a->k, "k", a->key_tokens, a->head_dim);
+  if (rc == FT_OK && a->key_tokens > 0) rc = check_apart(&a->v, "v", a->key_tokens, a->head_dim);
+  if (rc != FT_OK) return rc;
+  ServeAttentionParams p{};
+  p.q = static_cast<const uint16_t*>(a->q.data);
+  p.k = static_cast<const uint16_t*>(a->k.data);
+  p.v = static_cast<const uint16_t*>(a->v.data);
+  p.out = static_cast<uint16_t*>(a->out.data);
+  p.lse = a->lse;
+  p.q_token_stride = a->q.token_stride;
+  p.q_head_stride = a->q.head_stride;
+  p.out_token_stride = a->out.token_stride;
+  p.out_head_stride = a->out.head_stride;
+  p.kv_token_stride = a->k.token_stride;
+  p.kv_head_stride = a->k.head_stride;
+  p.v_token_stride = a->v.token_stride;
+  p.v_head_stride = a->v.head_stride;
+  p.q_offsets = a->q_offsets;
+  p.k_offsets = a->k_offsets != nullptr ? a->k_offsets : a->q_offsets;
+  p.batch = a->batch;
+  p.query_tokens = a->query_tokens;
+  p.key_tokens = a->key_tokens;
+  p.heads = a->q.heads;
+  p.kv_heads = a->k.heads;
+  p.group = a->q.heads / a->k.heads;
+  p.head_dim = a->head_dim;
+  p.causal = a->causal != 0;
+  p.scale_log2 = 1.44269504088896340736f * (a->scale != 0.0f ? a->scale : 1.0f / std::sqrt(static_cast<float>(a->head_dim)));
+  p.status = status;
+  SERVE_CUDA(launch_serve_attention(p, a->dtype, static_cast<cudaStream_t>(stream)));
+  return FT_OK;
+}
+
+int ft_tree_attention_run(const ft_kv_cache* cache, const ft_tree_attention_args* a, void* workspace, size_t workspace_bytes, int* status,
+                          void* stream) {
+  if (a == nullptr) return noalloc_fail(FT_ERR_INVALID, "null arguments");
+  int rc = check_cache(cache);
+  if (rc == FT_OK) rc = check_attention_call(workspace, workspace_bytes, status, a->q.heads, cache->kv_heads);
+  if (rc == FT_OK) rc = check_scale(a->scale);
+  if (rc != FT_OK) return rc;
+  if (a->layer < 0 || a->layer >= cache->layers) return noalloc_fail(FT_ERR_INVALID, "layer %d is outside the cache's %d", a->layer, cache->layers);
+  if (a->batch < 0 || a->query_tokens < 0) return noalloc_fail(FT_ERR_INVALID, "negative batch or token count");
+  if (a->table_pages <= 0 || a->table_stride < a->table_pages || a->table_pages > INT32_MAX / cache->page_size) {
+    return noalloc_fail(FT_ERR_INVALID, "the page table needs columns (below 2^31 tokens) and a stride that holds them (got %d, %d)", a->table_pages,
+                        a->table_stride);
+  }
+  if (a->mask != nullptr && (a->mask_words <= 0 || a->mask_stride < a->mask_words)) {
+    return noalloc_fail(FT_ERR_INVALID, "the mask needs words and a stride that holds them (got %d, %d)", a->mask_words, a->mask_stride);
+  }
+  if (a->batch == 0 || a->query_tokens == 0) return FT_OK;
+  if (a->q_offsets == nullptr || a->page_table == nullptr || a->lengths == nullptr) return noalloc_fail(FT_ERR_INVALID, "null q_offsets, page table or lengths");
+  rc = check_rows(&a->q, "q", a->q.heads);
+  if (rc == FT_OK) rc = check_rows(&a->out, "out", a->q.heads);
+  if (rc == FT_OK) rc = check_apart(&a->q, "q", a->query_tokens, cache->head_dim);
+  if (rc == FT_OK) rc = check_apart(&a->out, "out", a->query_tokens, cache->head_dim);
+  if (rc != FT_OK) return rc;
+  ServeAttentionParams p{};
+  p.q = static_cast<const uint16_t*>(a->q.data);
+  p.k = static_cast<const uint16_t*>(cache->k) + a->layer * cache->layer_stride;
+  p.v = static_cast<const uint16_t*>(cache->v) + a->layer * cache->layer_stride;
+  p.out = static_cast<uint16_t*>(a->out.data);
+  p.lse = a->lse;
+  p.q_token_stride = a->q.token_stride;
+  p.q_head_stride = a->q.head_stride;
+  p.out_token_stride = a->out.token_stride;
+  p.out_head_stride = a->out.head_stride;
+  p.kv_token_stride = p.v_token_stride = cache->token_stride;
+  p.kv_head_stride = p.v_head_stride = cache->head_stride;
+  p.page_stride = cache->page_stride;
+  p.q_offsets = a->q_offsets;
+  p.page_table = a->page_table;
+  p.lengths = a->lengths;
+  p.mask = a->mask;
+  p.mask_words = a->mask_words;
+  p.mask_stride = a->mask_stride;
+  p.batch = a->batch;
+  p.query_tokens = a->query_tokens;
+  p.heads = a->q.heads;
+  p.kv_heads = cache->kv_heads;
+  p.group = a->q.heads / cache->kv_heads;
+  p.head_dim = cache->head_dim;
+  p.causal = 1;
+  p.page_size = cache->page_size;
+  p.pages = cache->pages;
+  p.table_pages = a->table_pages;
+  p.table_stride = a->table_stride;
+  p.scale_log2 = 1.44269504088896340736f * (a->scale != 0.0f ? a->scale : 1.0f / std::sqrt(static_cast<float>(cache->head_dim)));
+  p.status = status;
+  SERVE_CUDA(launch_serve_attention(p, cache->dtype, static_cast<cudaStream_t>(stream)));
+  return FT_OK;
+}
+
+int ft_tree_mask(const int* parents, int nodes, uint32_t* mask, int words) {
+  if (nodes < 0 || words < 0 || (nodes > 0 && (parents == nullptr || mask == nullptr)) || nodes > static_cast<long long>(words) * 32) {
+    return noalloc_fail(FT_ERR_INVALID, "a tree of %d nodes needs parents and a mask of at least as many bits (%d words)", nodes, words);
+  }
+  for (int i = 0; i < nodes; ++i) {
+    if (parents[i] >= i) return noalloc_fail(FT_ERR_INVALID, "node %d has the parent %d: parents come before their children", i, parents[i]);
+    uint32_t* row = mask + static_cast<size_t>(i) * words;
+    if (parents[i] >= 0) {
+      std::copy(mask + static_cast<size_t>(parents[i]) * words, mask + static_cast<size_t>(parents[i] + 1) * words, row);
+    } else {
+      std::fill(row, row + words, 0u);
+    }
+    row[i / 32] |= 1u << (i % 32);
+  }
+  return FT_OK;
+}
+
+}  // extern "C"

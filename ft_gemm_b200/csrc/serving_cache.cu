@@ -1,0 +1,213 @@
+// Rotary positions and the page operations of the key/value cache: one pass over the
+// data each, bound by HBM for many tokens and by launch latency for few.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "serving_kernels.h"
+
+namespace ftg {
+
+namespace {
+
+__device__ __forceinline__ float2 unpack(__half2 v) { return __half22float2(v); }
+__device__ __forceinline__ float2 unpack(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+__device__ __forceinline__ void pack(__half2& d, float x, float y) { d = __floats2half2_rn(x, y); }
+__device__ __forceinline__ void pack(__nv_bfloat162& d, float x, float y) { d = __floats2bfloat162_rn(x, y); }
+
+template <typename T>
+union Chunk {  // 16 bytes: eight elements
+  uint4 raw;
+  T pairs[4];
+};
+
+constexpr int kRotaryThreads = 256;
+
+// Rotates, copies and scatters the rows of `tokens_per_block` tokens.  A thread takes two 16-byte chunks of one row: the
+// two halves of eight pairs (or, interleaved, eight pairs outright), or two chunks that are only copied.  Sines and cosines
+// are computed once per token and frequency, shared by all heads: the angle in turns is position * frequency / 2pi, formed
+// and reduced to [-1/2, 1/2] in 64 bits (32 bits lose it beyond some ten thousand positions), then one sincospi in 32 bits.
+template <typename T>
+__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryParams p, int tokens_per_block) {
+  extern __shared__ float2 turn[];  // [token in block][rotary_dim / 2]: magnitude * (cos, sin)
+  const int half = p.rotary_dim / 2;
+  const int first = blockIdx.x * tokens_per_block;
+  const int count = min(tokens_per_block, p.tokens - first);
+  const int thread = threadIdx.y * blockDim.x + threadIdx.x;
+  for (int i = thread; i < count * half; i += blockDim.x * blockDim.y) {
+    const int t = i / half, f = i - t * half;
+    double angle = static_cast<double>(p.positions[first + t]) * p.turns[f];
+    angle -= rint(angle);
+    float s, c;
+    sincospif(2.0f * static_cast<float>(angle), &s, &c);
+    turn[i] = make_float2(c * p.magnitude, (p.inverse ? -s : s) * p.magnitude);
+  }
+  __syncthreads();
+
+  const int rows = p.q_heads + p.k_heads + p.v_heads;
+  const int unit = threadIdx.x;  // which two chunks of the row
+  const int rotated_units = p.rotary_dim / 16;
+  for (int r = threadIdx.y; r < count * rows; r += blockDim.y) {
+    const int t = r / rows;
+    int head = r - t * rows;
+    const long long token = first + t;
+    const uint16_t* src;
+    uint16_t* dst;
+    bool rotate = unit < rotated_units;
+    if (head < p.q_heads) {
+      src = p.q.data + token * p.q.token_stride + head * p.q.head_stride;
+      dst = p.q_out.data + token * p.q_out.token_stride + head * p.q_out.head_stride;
+    } else {
+      head -= p.q_heads;
+      const bool value = head >= p.k_heads;
+      if (value) {
+        head -= p.k_heads;
+        rotate = false;
+      }
+      const Rows& rows_in = value ? p.v : p.k;
+      src = rows_in.data + token * rows_in.token_stride + head * rows_in.head_stride;
+      if (p.slots != nullptr) {
+        const long long slot = p.slots[token];
+        if (slot < 0 || slot >= p.slot_count) continue;  // padding of the batch
+        dst = (value ? p.v_cache : p.k_cache) + (slot / p.page_size) * p.page_stride + (slot % p.page_size) * p.cache_token_stride +
+              head * p.cache_head_stride;
+      } else {
+        dst = p.k_out.data + token * p.k_out.token_stride + head * p.k_out.head_stride;
+      }
+    }
+    const bool halves = rotate && !p.interleaved;
+    const int at0 = halves ? unit * 8 : unit * 16, at1 = halves ? at0 + half : at0 + 8;
+    Chunk<T> a, b;
+    a.raw = *reinterpret_cast<const uint4*>(src + at0);
+    b.raw = *reinterpret_cast<const uint4*>(src + at1);
+    if (rotate) {
+      const float2* cs = turn + t * half + unit * 8;
+      if (p.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 x = unpack(a.pairs[i]), y = unpack(b.pairs[i]);
+          const float2 u = cs[i], w = cs[4 + i];
+          pack(a.pairs[i], x.x * u.x - x.y * u.y, x.x * u.y + x.y * u.x);
+          pack(b.pairs[i], y.x * w.x - y.y * w.y, y.x * w.y + y.y * w.x);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 x = unpack(a.pairs[i]), y = unpack(b.pairs[i]);
+          const float2 u = cs[2 * i], w = cs[2 * i + 1];
+          pack(a.pairs[i], x.x * u.x - y.x * u.y, x.y * w.x - y.y * w.y);
+          pack(b.pairs[i], x.x * u.y + y.x * u.x, x.y * w.y + y.y * w.x);
+        }
+      }
+    }
+    *reinterpret_cast<uint4*>(dst + at0) = a.raw;
+    *reinterpret_cast<uint4*>(dst + at1) = b.raw;
+  }
+}
+
+// Whole pages, a block for each 16 KiB piece of one page of one layer, of K or of V.
+constexpr int kCopyThreads = 256, kCopyUnroll = 4;
+
+__global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const CopyPagesParams p, int pieces) {
+  const int pair = blockIdx.x / pieces, piece = blockIdx.x - pair * pieces;
+  const int source = p.sources[pair], target = p.targets[pair];
+  if (source < 0 || source >= p.pages || target < 0 || target >= p.pages || source == target) return;
+  uint16_t* base = (blockIdx.y & 1 ? p.v : p.k) + (blockIdx.y >> 1) * p.layer_stride;
+  const uint4* src = reinterpret_cast<const uint4*>(base + source * p.page_stride);
+  uint4* dst = reinterpret_cast<uint4*>(base + target * p.page_stride);
+  const int chunks = p.page_elements / 8;
+  const int at = piece * kCopyThreads * kCopyUnroll + threadIdx.x;
+  uint4 x[kCopyUnroll];
+#pragma unroll
+  for (int i = 0; i < kCopyUnroll; ++i) {
+    if (at + i * kCopyThreads < chunks) x[i] = __ldcs(src + at + i * kCopyThreads);
+  }
+#pragma unroll
+  for (int i = 0; i < kCopyUnroll; ++i) {
+    if (at + i * kCopyThreads < chunks) __stcs(dst + at + i * kCopyThreads, x[i]);
+  }
+}
+
+// Compaction of the accepted drafted tokens: a block for one sequence, one layer, and K or V; a thread owns some 16-byte
+// columns of the rows and carries every accepted token's column to its new place, eight at a time.  Places ascend and none
+// lies behind its source, so a column that was read has been read before it is overwritten, whatever else the block does.
+constexpr int kAcceptBatch = 8, kAcceptTile = 64;
+
+__global__ void __launch_bounds__(256) accept_kernel(const AcceptParams p) {
+  __shared__ long long from[kAcceptTile], to[kAcceptTile];
+  const int b = blockIdx.x;
+  const int drafted = p.drafted_offsets[b + 1] - p.drafted_offsets[b];
+  const int base = p.lengths[b] - drafted;
+  const int begin = p.accepted_offsets[b], count = p.accepted_offsets[b + 1] - begin;
+  if (blockIdx.y == 0 && threadIdx.x == 0) p.new_lengths[b] = base + max(count, 0);
+  uint16_t* cache = (blockIdx.y & 1 ? p.v : p.k) + (blockIdx.y >> 1) * p.layer_stride;
+  const int row_chunks = p.head_dim / 8, columns = p.kv_heads * row_chunks;
+  for (int tile = 0; tile < count; tile += kAcceptTile) {
+    const int here = min(kAcceptTile, count - tile);
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * here; i += blockDim.x) {
+      const int at = tile + i / 2;
+      const int node = i & 1 ? at : p.accepted[begin + at];
+      const int place = base + node;
+      long long offset = -1;
+      if (node >= 0 && node < drafted && place >= 0 && place / p.page_size < p.table_pages) {
+        const int page = p.page_table[static_cast<long long>(b) * p.table_stride + place / p.page_size];
+        if (page >= 0 && page < p.pages) offset = page * p.page_stride + (place % p.page_size) * p.token_stride;
+      }
+      (i & 1 ? to : from)[i / 2] = offset;
+    }
+    __syncthreads();
+    for (int column = threadIdx.x; column < columns; column += blockDim.x) {
+      const int head = column / row_chunks;
+      uint16_t* mine = cache + head * p.head_stride + (column - head * row_chunks) * 8;
+      for (int i0 = 0; i0 < here; i0 += kAcceptBatch) {
+        uint4 x[kAcceptBatch];
+#pragma unroll
+        for (int i = 0; i < kAcceptBatch; ++i) {
+          if (i0 + i < here && from[i0 + i] >= 0) x[i] = *reinterpret_cast<const uint4*>(mine + from[i0 + i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kAcceptBatch; ++i) {
+          if (i0 + i < here && from[i0 + i] >= 0 && to[i0 + i] >= 0 && from[i0 + i] != to[i0 + i]) {
+            *reinterpret_cast<uint4*>(mine + to[i0 + i]) = x[i];
+          }
+        }
+      }
+    }
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_rotary(const RotaryParams& p, int dtype, cudaStream_t stream) {
+  const int rows = p.q_heads + p.k_heads + p.v_heads;
+  if (p.tokens <= 0 || rows <= 0) return cudaSuccess;
+  const dim3 block(p.head_dim / 16, kRotaryThreads / (p.head_dim / 16));
+  const int tokens_per_block = std::min(16, std::max(1, static_cast<int>(block.y) / rows));
+  const int grid = (p.tokens + tokens_per_block - 1) / tokens_per_block;
+  const size_t smem = static_cast<size_t>(tokens_per_block) * (p.rotary_dim / 2) * sizeof(float2);
+  if (dtype == FT_SRC_BF16) {
+    rotary_kernel<__nv_bfloat162><<<grid, block, smem, stream>>>(p, tokens_per_block);
+  } else {
+    rotary_kernel<__half2><<<grid, block, smem, stream>>>(p, tokens_per_block);
+  }
+  return cudaGetLastError();
+}
+
+cudaError_t launch_copy_pages(const CopyPagesParams& p, cudaStream_t stream) {
+  if (p.count <= 0) return cudaSuccess;
+  const int pieces = (p.page_elements / 8 + kCopyThreads * kCopyUnroll - 1) / (kCopyThreads * kCopyUnroll);
+  copy_pages_kernel<<<dim3(static_cast<unsigned>(p.count) * pieces, 2 * p.layers), kCopyThreads, 0, stream>>>(p, pieces);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_accept(const AcceptParams& p, cudaStream_t stream) {
+  if (p.batch <= 0) return cudaSuccess;
+  const int columns = p.kv_heads * p.head_dim / 8;
+  const int threads = std::min(256, (columns + 31) / 32 * 32);
+  accept_kernel<<<dim3(p.batch, 2 * p.layers), threads, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace ftg

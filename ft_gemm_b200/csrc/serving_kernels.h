@@ -1,0 +1,70 @@
+// Internal interface between the serving C-ABI (api_serving.cu) and its kernels.
+#pragma once
+#include <cuda_runtime.h>
+
+#include "../../include/ft_serving.h"
+
+namespace ftg {
+
+struct Rows {  // ft_rows with 16-bit elements
+  uint16_t* data;
+  long long token_stride, head_stride;
+};
+
+// One pass over the rows of a token: rotates q and k (or copies them where rotary_dim ends), writes k and v to pages.
+struct RotaryParams {
+  Rows q, q_out, k, k_out, v;
+  int q_heads, k_heads, v_heads;  // v_heads: k_heads when K and V go to the cache, else 0
+  const double* turns;            // frequencies in turns per position, rotary_dim / 2 of them
+  const long long* positions;
+  const long long* slots;  // with the cache: where k and v go
+  uint16_t *k_cache, *v_cache;
+  long long page_stride, cache_token_stride, cache_head_stride;
+  long long slot_count;
+  int page_size;
+  int tokens, head_dim, rotary_dim;
+  int interleaved, inverse;
+  float magnitude;
+};
+cudaError_t launch_rotary(const RotaryParams& params, int dtype, cudaStream_t stream);
+
+struct CopyPagesParams {
+  uint16_t *k, *v;
+  long long layer_stride, page_stride;
+  int layers, pages, page_elements, count;
+  const int *sources, *targets;
+};
+cudaError_t launch_copy_pages(const CopyPagesParams& params, cudaStream_t stream);
+
+struct AcceptParams {
+  uint16_t *k, *v;
+  long long layer_stride, page_stride, token_stride, head_stride;
+  int layers, pages, page_size, kv_heads, head_dim;
+  const int *page_table, *lengths, *drafted_offsets, *accepted, *accepted_offsets;
+  int table_pages, table_stride, batch;
+  int* new_lengths;
+};
+cudaError_t launch_accept(const AcceptParams& params, cudaStream_t stream);
+
+// Attention of the queries of each sequence over its keys: packed prompts (page_table == nullptr) or the paged cache.
+struct ServeAttentionParams {
+  const uint16_t *q, *k, *v;
+  uint16_t* out;
+  float* lse;
+  long long q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  long long kv_token_stride, kv_head_stride, v_token_stride, v_head_stride, page_stride;
+  const int* q_offsets;
+  const int* k_offsets;   // packed prompts
+  const int* page_table;  // paged cache
+  const int* lengths;
+  const uint32_t* mask;
+  int mask_words, mask_stride;
+  int batch, query_tokens, key_tokens;
+  int heads, kv_heads, group, head_dim, causal;
+  int page_size, pages, table_pages, table_stride;
+  float scale_log2;  // log2(e) * scale
+  int* status;
+};
+cudaError_t launch_serve_attention(const ServeAttentionParams& params, int dtype, cudaStream_t stream);
+
+}  // namespace ftg

@@ -1,0 +1,263 @@
+"""CPU checks of the serving operators (include/ft_serving.h): refusals before any CUDA call, rotary frequencies, tree
+masks and the page pool, which are host functions."""
+import ctypes
+import math
+import os
+import random
+import re
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HEADER = os.path.join(ROOT, "include", "ft_serving.h")
+
+
+@pytest.fixture(scope="module")
+def ftg(lib_path):
+    import ft_gemm_b200
+    return ft_gemm_b200
+
+
+@pytest.fixture(scope="module")
+def sv(ftg):
+    from ft_gemm_b200 import serving
+    serving._lib()
+    return serving
+
+
+def test_library_exports_every_declared_symbol(lib_path):
+    text = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+    names = set(re.findall(r"\b(ft_[a-z0-9_]+)\s*\(", text))
+    assert {"ft_rotary_run", "ft_kv_cache_append", "ft_prompt_attention_run", "ft_tree_attention_run"} <= names
+    out = subprocess.run(["nm", "-D", "--defined-only", lib_path], capture_output=True, text=True, check=True).stdout
+    for name in names:
+        assert re.search(rf"\bT {name}\b", out), name
+
+
+def test_header_is_c_and_struct_sizes_match(tmp_path, sv):
+    src = tmp_path / "s.c"
+    names = ["ft_rows", "ft_rotary_options", "ft_kv_cache", "ft_prompt_attention_args", "ft_tree_attention_args"]
+    src.write_text('#include <stdio.h>\n#include "ft_serving.h"\nint main(void){printf("' + "%zu " * len(names) + '\\n", '
+                   + ", ".join(f"sizeof({n})" for n in names) + "); return 0;}\n")
+    subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(tmp_path / "s")], check=True)
+    sizes = [int(x) for x in subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout.split()]
+    assert sizes == [ctypes.sizeof(t) for t in (sv.FtRows, sv.FtRotaryOptions, sv.FtKvCache, sv.FtPromptAttentionArgs, sv.FtTreeAttentionArgs)]
+
+
+def _frequencies(sv, **fields):
+    o = sv.FtRotaryOptions()
+    sv._lib().ft_rotary_options_default(ctypes.byref(o), fields.pop("head_dim", 128))
+    for name, value in fields.items():
+        setattr(o, name, value)
+    out = (ctypes.c_double * 128)()
+    return sv._lib().ft_rotary_frequencies(ctypes.byref(o), out), list(out[:max(0, min(256, o.rotary_dim)) // 2])
+
+
+@pytest.mark.parametrize("scaling", [0, 1, 2, 3])
+def test_rotary_frequencies(sv, ftg, scaling):
+    code, got = _frequencies(sv, rotary_dim=96, scaling=scaling, base=500000.0, factor=8.0, original_length=8192.0)
+    assert code == ftg.FT_OK
+    for i, g in enumerate(got):
+        f = math.exp(-2 * i / 96 * math.log(500000.0 * (8 ** (96 / 94) if scaling == 2 else 1)))
+        if scaling == 1:
+            f /= 8
+        if scaling == 3:
+            turns = 8192 * f / (2 * math.pi)
+            keep = 1.0 if turns >= 4 else 0.0 if turns <= 1 else (turns - 1) / 3
+            f = f * keep + f / 8 * (1 - keep)
+        assert g == pytest.approx(f, rel=1e-13)
+
+
+def test_rotary_refusals(sv, ftg):
+    for bad in (dict(rotary_dim=0), dict(rotary_dim=24), dict(rotary_dim=144), dict(head_dim=72), dict(head_dim=512), dict(base=0.0),
+                dict(base=math.nan), dict(factor=0.0), dict(factor=-1.0), dict(magnitude=math.inf), dict(scaling=4), dict(scaling=-1),
+                dict(scaling=3), dict(scaling=3, original_length=8192.0, low=4.0, high=4.0)):
+        assert _frequencies(sv, **bad)[0] == ftg.FT_ERR_INVALID, bad
+    lib, rows = sv._lib(), sv.FtRows(0x1000, 128, 128, 1)
+    assert lib.ft_rotary_run(None, rows, rows, None, None, None, 1, 1, 0, None) == ftg.FT_ERR_INVALID
+    assert lib.ft_rotary_prepare(None, None, None) == ftg.FT_ERR_INVALID
+    assert lib.ft_rotary_destroy(None) == ftg.FT_OK
+
+
+def _cache(sv, **fields):
+    c = sv.FtKvCache(0x10000, 0x20000, 2 * 4 * 16 * 2 * 64, 16 * 2 * 64, 2 * 64, 64, 2, 4, 16, 2, 64, 1)
+    for name, value in fields.items():
+        setattr(c, name, value)
+    return c
+
+
+def test_cache_refusals(sv, ftg):
+    lib = sv._lib()
+    assert lib.ft_kv_cache_copy_pages(_cache(sv), None, None, 0, None) == ftg.FT_OK
+    for bad in (dict(k=None), dict(v=None), dict(k=0x10008), dict(dtype=0), dict(layers=0), dict(pages=0), dict(kv_heads=0), dict(head_dim=96),
+                dict(page_size=24), dict(page_size=4), dict(page_size=512), dict(token_stride=64), dict(head_stride=128), dict(page_stride=2047),
+                dict(page_stride=1024), dict(layer_stride=8193)):
+        assert lib.ft_kv_cache_copy_pages(_cache(sv, **bad), None, None, 0, None) == ftg.FT_ERR_INVALID, bad
+    assert lib.ft_kv_cache_copy_pages(None, None, None, 0, None) == ftg.FT_ERR_INVALID
+    assert lib.ft_kv_cache_copy_pages(_cache(sv), None, None, 1, None) == ftg.FT_ERR_INVALID
+    assert lib.ft_kv_cache_copy_pages(_cache(sv), 0x1000, 0x1000, -1, None) == ftg.FT_ERR_INVALID
+    # by head: a page [kv_heads][page_size][head_dim]
+    assert lib.ft_kv_cache_copy_pages(_cache(sv, token_stride=64, head_stride=16 * 64), None, None, 0, None) == ftg.FT_OK
+    good = sv.FtRows(0x1000, 128, 64, 2)
+    for k, v, slots, layer, rotary, q in ((None, good, 0x1000, 0, None, None), (good, None, 0x1000, 0, None, None), (good, good, None, 0, None, None),
+                                          (good, good, 0x1000, 2, None, None), (good, good, 0x1000, -1, None, None),
+                                          (good, good, 0x1000, 0, None, good), (sv.FtRows(0x1000, 128, 64, 3), good, 0x1000, 0, None, None),
+                                          (sv.FtRows(0x1004, 128, 64, 2), good, 0x1000, 0, None, None),
+                                          (sv.FtRows(0x1000, 130, 64, 2), good, 0x1000, 0, None, None)):
+        assert lib.ft_kv_cache_append(_cache(sv), layer, k, v, slots, 1, rotary, None, q, q, None) == ftg.FT_ERR_INVALID
+    x = 0x1000
+    assert lib.ft_kv_cache_accept(_cache(sv), x, 4, 4, x, x, x, x, 1, x, None) == ftg.FT_ERR_INVALID and b"lengths array" in lib.ft_gemm_last_error()
+    assert lib.ft_kv_cache_accept(_cache(sv), x, 4, 3, x, x, x, x, 1, x + 64, None) == ftg.FT_ERR_INVALID
+    assert lib.ft_kv_cache_accept(_cache(sv), None, 4, 4, x, x, x, x, 1, x + 64, None) == ftg.FT_ERR_INVALID
+
+
+def test_attention_refusals(sv, ftg):
+    lib = sv._lib()
+    size = 1 << 40  # of the workspace, said only
+
+    def prompt(workspace=0x100000, status=0x1000, **fields):
+        r = lambda heads: sv.FtRows(0x10000, heads * 128, 128, heads)  # noqa: E731
+        a = sv.FtPromptAttentionArgs(r(8), r(2), r(2), r(8), None, 0x1000, None, 1, 16, 16, 128, 1, 1, 0.0)
+        for name, value in fields.items():
+            setattr(a, name, value)
+        return lib.ft_prompt_attention_run(a, workspace, size, status, None)
+
+    rows = sv.FtRows
+    for bad in (dict(workspace=None), dict(workspace=0x100008), dict(status=None), dict(dtype=0), dict(dtype=3), dict(head_dim=96), dict(head_dim=256),
+                dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(batch=-1), dict(query_tokens=-1), dict(q_offsets=None),
+                dict(q=rows(0x10000, 1024, 128, 7)), dict(q=rows(0x10000, 1024, 128, 0)), dict(q=rows(0x10000, 65 * 512, 128, 258)),
+                dict(q=rows(None, 1024, 128, 8)), dict(q=rows(0x10002, 1024, 128, 8)), dict(k=rows(0x10000, 257, 128, 2)),
+                dict(v=rows(0x10000, 256, 128, 3)), dict(out=rows(0x10000, 1024, 128, 4)), dict(out=rows(0x10000, 1024, 4, 8))):
+        assert prompt(**bad) == ftg.FT_ERR_INVALID, bad
+    assert lib.ft_prompt_attention_run(None, 0x100000, size, 0x1000, None) == ftg.FT_ERR_INVALID
+    assert prompt(batch=0) == ftg.FT_OK and prompt(query_tokens=0) == ftg.FT_OK
+
+    def tree(cache=None, workspace=0x100000, bytes_=size, status=0x1000, **fields):
+        r = sv.FtRows(0x10000, 4 * 64, 64, 4)
+        a = sv.FtTreeAttentionArgs(r, r, None, 0x1000, 0x1000, 0x1000, None, 0, 0, 1, 4, 4, 4, 0, 0.0)
+        for name, value in fields.items():
+            setattr(a, name, value)
+        return lib.ft_tree_attention_run(cache or _cache(sv), a, workspace, bytes_, status, None)
+
+    for bad in (dict(cache=_cache(sv, page_size=12)), dict(workspace=None), dict(bytes_=0), dict(status=None), dict(layer=2), dict(layer=-1),
+                dict(table_pages=0), dict(table_stride=3), dict(table_pages=1 << 28, table_stride=1 << 28), dict(mask=0x1000), dict(mask=0x1000, mask_words=2, mask_stride=1),
+                dict(batch=-1), dict(q_offsets=None), dict(page_table=None), dict(lengths=None), dict(scale=-0.5),
+                dict(q=rows(0x10000, 192, 64, 3)), dict(out=rows(0x10008, 256, 64, 4))):
+        assert tree(**bad) == ftg.FT_ERR_INVALID, bad
+    assert tree(batch=0) == ftg.FT_OK
+
+
+def test_python_refuses_what_is_not_a_cuda_cache(ftg):
+    torch = pytest.importorskip("torch")
+    k = torch.empty((1, 2, 16, 2, 64), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        ftg.PagedCache(k, k.clone())
+    with pytest.raises(ValueError, match="scaling"):
+        ftg.Rotary(128, scaling="by parts")
+    with pytest.raises(ftg.FtGemmError, match="multiples of 16"):
+        ftg.Rotary(128, rotary_dim=40)
+    with pytest.raises(ValueError, match="element type"):
+        ftg.PromptAttention(8, 2, 128, dtype=torch.float32)
+
+
+def test_tree_mask(ftg):
+    pytest.importorskip("torch")
+    rng = random.Random(3)
+    for nodes, words in ((0, 0), (1, None), (33, None), (70, 4)):
+        parents = [rng.randint(-1, i - 1) for i in range(nodes)]
+        got = ftg.tree_mask(parents, words)
+        for i in range(nodes):
+            want, j = set(), i
+            while j >= 0:
+                want.add(j)
+                j = parents[j]
+            row = [int(w) & 0xFFFFFFFF for w in got[i]]
+            assert {j for j in range(32 * len(row)) if row[j // 32] >> (j % 32) & 1} == want
+    with pytest.raises(ftg.FtGemmError, match="before their children"):
+        ftg.tree_mask([-1, 1])
+    with pytest.raises(ftg.FtGemmError, match="bits"):
+        ftg.tree_mask([-1] * 33, 1)
+
+
+def test_page_pool_against_a_model(ftg):
+    """Random calls; the contents of every page are modelled on the side, and pages are copied as the pool says."""
+    pytest.importorskip("torch")
+    rng = random.Random(11)
+    for size, pages in ((1, 30), (4, 24), (16, 9)):
+        pool, store, want, token = ftg.PagePool(pages, size), [[None] * size for _ in range(pages)], {}, 0
+        for _ in range(600):
+            act = rng.choice(["new", "extend", "extend", "extend", "fork", "free", "truncate", "compact"])
+            some = rng.choice(list(want)) if want else None
+            if act == "new" and len(want) < 8:
+                want[pool.new_sequence()] = []
+            elif some is None:
+                continue
+            elif act == "extend":
+                count, free = rng.randint(0, 2 * size + 1), pool.free_pages()
+                before = pool.page_list(some)
+                try:
+                    pairs = pool.extend([some], [count])
+                except ftg.FtGemmError:
+                    assert pool.free_pages() == free and pool.page_list(some) == before and pool.length(some) == len(want[some])
+                    continue
+                for a, b in pairs:
+                    store[b] = list(store[a])
+                first = len(want[some])
+                for slot in pool.slots(some, first, count):
+                    store[slot // size][slot % size] = token
+                    want[some].append(token)
+                    token += 1
+            elif act == "fork" and len(want) < 8:
+                want[pool.fork(some)] = list(want[some])
+            elif act == "free":
+                pool.free(some)
+                del want[some]
+            elif act == "truncate":
+                length = rng.randint(0, len(want[some]))
+                pool.truncate(some, length)
+                del want[some][length:]
+            elif act == "compact":
+                pairs = pool.compact()
+                assert not {a for a, _ in pairs} & {b for _, b in pairs}
+                for a, b in pairs:
+                    store[b] = list(store[a])
+            used = {p for s in want for p in pool.page_list(s)}
+            assert pool.free_pages() == pages - len(used)
+            if act == "compact":
+                assert used == set(range(len(used)))
+            for s, tokens in want.items():
+                assert pool.length(s) == len(tokens)
+                assert [store[x // size][x % size] for x in pool.slots(s, 0, len(tokens))] == tokens
+        for s in list(want):
+            pool.free(s)
+        assert pool.free_pages() == pages
+        with pytest.raises(ftg.FtGemmError, match="no sequence"):
+            pool.free(0)
+        with pytest.raises(ftg.FtGemmError):
+            pool.fork(-1)
+        pool.close()
+
+
+def test_page_pool_refusals(ftg, sv):
+    pytest.importorskip("torch")
+    lib, handle = sv._lib(), ctypes.c_void_p()
+    assert lib.ft_page_pool_create(ctypes.byref(handle), 0, 16) == ftg.FT_ERR_INVALID
+    assert lib.ft_page_pool_create(ctypes.byref(handle), 4, 0) == ftg.FT_ERR_INVALID
+    assert lib.ft_page_pool_create(None, 4, 16) == ftg.FT_ERR_INVALID
+    assert lib.ft_page_pool_free_pages(None) == ftg.FT_ERR_INVALID
+    assert lib.ft_page_pool_destroy(None) == ftg.FT_OK
+    pool = ftg.PagePool(4, 16)
+    s = pool.new_sequence()
+    with pytest.raises(ftg.FtGemmError, match="free pages"):
+        pool.extend([s], [65])
+    with pytest.raises(ftg.FtGemmError):
+        pool.extend([s], [-1])
+    with pytest.raises(ftg.FtGemmError):
+        pool.extend([s], [2 ** 31 - 1])
+    with pytest.raises(ftg.FtGemmError):
+        pool.truncate(s, 1)
+    with pytest.raises(ValueError):
+        pool.slots(s, 0, 1)
+    with pytest.raises(ValueError):
+        pool.extend([s], [1, 2])
