@@ -9,7 +9,7 @@ NVCCFLAGS ?= -O3 -std=c++17 -lineinfo $(ARCH) -Xcompiler -fPIC -Xptxas -v
 CSRC      := ft_gemm_b200/csrc
 LIB       := ft_gemm_b200/lib/libft_gemm_b200.so
 OBJS      := build/obj/prepare.o build/obj/prepare_mma.o build/obj/abft_gemm.o build/obj/api.o build/obj/noalloc.o build/obj/ft_attention.o build/obj/ft_attention_split.o build/obj/api_attention.o build/obj/gemm_softmax.o build/obj/serving_cache.o build/obj/serving_attention.o build/obj/api_serving.o
-HDRS      := include/ft_gemm.h include/ft_attention.h include/ft_gemm_softmax.h include/ft_serving.h $(CSRC)/serving_kernels.h $(CSRC)/kernels.h $(CSRC)/attention_kernels.h $(CSRC)/attention_device.cuh $(CSRC)/abft_tile_check.cuh $(CSRC)/sm100_ptx.cuh
+HDRS      := include/ft_gemm.h include/ft_attention.h include/ft_gemm_softmax.h include/ft_serving.h $(CSRC)/serving_kernels.h $(CSRC)/serving_schedule.h $(CSRC)/kernels.h $(CSRC)/attention_kernels.h $(CSRC)/attention_device.cuh $(CSRC)/abft_tile_check.cuh $(CSRC)/sm100_ptx.cuh
 
 # the campaign the 100 % single-fault correction claim is quoted on: 8192^3, N(0,1) inputs, 1000 single faults U[1,256]
 # with random sign + 50 double faults, relative tolerance 2e-6 (the reference's default 2e-5 puts the threshold near 6.7

@@ -2,6 +2,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <new>
@@ -80,12 +81,63 @@ int check_scale(float scale) {
   return FT_OK;
 }
 
-int check_device() {
-  int device = 0, major = 0;
+// The current device has to be an sm_100; its SM count, asked for once per device.
+int check_device(int* sm_count) {
+  static std::atomic<int> known[64];
+  int device = 0;
   SERVE_CUDA(cudaGetDevice(&device));
-  SERVE_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
-  if (major != 10) return noalloc_fail(FT_ERR_UNSUPPORTED, "this library needs an sm_100 GPU (found compute capability %d)", major);
+  int count = device < 64 ? known[device].load(std::memory_order_relaxed) : 0;
+  if (count == 0) {
+    int major = 0;
+    SERVE_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
+    if (major != 10) return noalloc_fail(FT_ERR_UNSUPPORTED, "this library needs an sm_100 GPU (found compute capability %d)", major);
+    SERVE_CUDA(cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device));
+    if (device < 64) known[device].store(count, std::memory_order_relaxed);
+  }
+  if (sm_count != nullptr) *sm_count = count;
   return FT_OK;
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// A 16-bit tensor, dims and boxes innermost first, strides in elements from the second dimension on; 128-byte swizzle, zeros
+// outside.  The dimensions that hold one element only may come with any stride.
+int make_map(CUtensorMap* map, int dtype, const void* base, int rank, const long long* dims, const long long* strides, const int* boxes) {
+  static std::atomic<EncodeTiledFn> known{nullptr};
+  EncodeTiledFn encode = known.load(std::memory_order_relaxed);
+  if (encode == nullptr) {
+    void* sym = nullptr;
+    cudaDriverEntryPointQueryResult query;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &query) != cudaSuccess || query != cudaDriverEntryPointSuccess) {
+      return noalloc_fail(FT_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    }
+    encode = reinterpret_cast<EncodeTiledFn>(sym);
+    known.store(encode, std::memory_order_relaxed);
+  }
+  cuuint64_t d[5], s[4];
+  cuuint32_t box[5], step[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = static_cast<cuuint64_t>(dims[i]);
+    box[i] = static_cast<cuuint32_t>(boxes[i]);
+    step[i] = 1;
+    if (i > 0) s[i - 1] = static_cast<cuuint64_t>(dims[i] > 1 ? strides[i - 1] : dims[0]) * 2;
+  }
+  const CUresult r = encode(map, dtype == FT_SRC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, static_cast<cuuint32_t>(rank),
+                            const_cast<void*>(base), d, s, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    return noalloc_fail(FT_ERR_INVALID, "the strides or sizes of a tensor are outside what the copy engine takes (CUresult %d)", static_cast<int>(r));
+  }
+  return FT_OK;
+}
+
+int make_query_map(CUtensorMap* map, int dtype, const ft_rows& q, int tokens, int kv_heads, int head_dim) {
+  const int group = q.heads / kv_heads;
+  const long long dims[4] = {head_dim, group, kv_heads, tokens}, strides[3] = {q.head_stride, group * q.head_stride, q.token_stride};
+  const int boxes[4] = {64, group, 1, 128 / group};
+  return make_map(map, dtype, q.data, 4, dims, strides, boxes);
 }
 
 }  // namespace
@@ -180,7 +232,7 @@ int ft_rotary_prepare(ft_rotary_handle** handle, const ft_rotary_options* option
   *handle = nullptr;
   double turns[128];
   int rc = ft_rotary_frequencies(options, turns);
-  if (rc == FT_OK) rc = check_device();
+  if (rc == FT_OK) rc = check_device(nullptr);
   if (rc != FT_OK) return rc;
   const int count = options->rotary_dim / 2;
   for (int i = 0; i < count; ++i) turns[i] /= 6.283185307179586476925286766559;
@@ -518,22 +570,54 @@ int ft_page_pool_compact(ft_page_pool* pool, int* sources, int* targets, int cap
 
 // ---- attention -------------------------------------------------------------------
 
-size_t ft_attention_workspace(void) { return 16; }
+size_t ft_attention_workspace(void) {
+  int sm_count = 0;
+  return check_device(&sm_count) == FT_OK ? serve_attention_workspace(sm_count) : 0;
+}
 
-static int check_attention_call(const void* workspace, size_t workspace_bytes, const int* status, int group_heads, int kv_heads) {
-  if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < ft_attention_workspace()) {
-    return noalloc_fail(FT_ERR_INVALID, "the workspace must be 16-byte aligned and hold ft_attention_workspace() bytes (%zu given)", workspace_bytes);
+static int check_heads(int heads, int kv_heads) {
+  if (kv_heads <= 0 || heads <= 0 || heads % kv_heads != 0 || heads / kv_heads > 128) {
+    return noalloc_fail(FT_ERR_INVALID, "query heads (%d) must be 1 to 128 times the key heads (%d)", heads, kv_heads);
   }
+  return FT_OK;
+}
+
+static int check_workspace(const void* workspace, size_t bytes, const int* status) {
+  if (workspace == nullptr || bytes == 0 || !aligned16(workspace)) return noalloc_fail(FT_ERR_INVALID, "the workspace must be there and 16-byte aligned");
   if (status == nullptr) return noalloc_fail(FT_ERR_INVALID, "null status");
-  if (kv_heads <= 0 || group_heads <= 0 || group_heads % kv_heads != 0 || group_heads / kv_heads > 128) {
-    return noalloc_fail(FT_ERR_INVALID, "query heads (%d) must be 1 to 128 times the key heads (%d)", group_heads, kv_heads);
+  return FT_OK;
+}
+
+// What both calls share: the rows of q and out, the launch.
+static int attention_run(ServeAttentionParams& p, const ft_rows& q, const ft_rows& out, const CUtensorMap& k_map, const CUtensorMap& v_map, int dtype,
+                         float scale, void* workspace, size_t workspace_bytes, int* status, int sm_count, void* stream) {
+  if (workspace_bytes < serve_attention_workspace(sm_count)) {
+    return noalloc_fail(FT_ERR_INVALID, "the workspace holds %zu bytes, ft_attention_workspace() says %zu", workspace_bytes,
+                        serve_attention_workspace(sm_count));
   }
+  CUtensorMap q_map;
+  const int rc = make_query_map(&q_map, dtype, q, p.query_tokens, p.kv_heads, p.head_dim);
+  if (rc != FT_OK) return rc;
+  p.out = static_cast<uint16_t*>(out.data);
+  p.out_token_stride = out.token_stride;
+  p.out_head_stride = out.head_stride;
+  p.heads = q.heads;
+  p.group = q.heads / p.kv_heads;
+  p.scale_log2 = 1.44269504088896340736f * (scale != 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(p.head_dim)));
+  p.min_share = 1;
+  p.workspace = workspace;
+  p.status = status;
+  // Two row tiles per CTA halve the reads of K and V, which pays once there are enough row tiles for every SM.
+  const long long pairs = (static_cast<long long>(p.query_tokens) * p.group + 255) / 256 * p.kv_heads;
+  const bool split_keys = pairs < sm_count;
+  SERVE_CUDA(launch_serve_attention(q_map, k_map, v_map, p, dtype, split_keys, sm_count, static_cast<cudaStream_t>(stream)));
   return FT_OK;
 }
 
 int ft_prompt_attention_run(const ft_prompt_attention_args* a, void* workspace, size_t workspace_bytes, int* status, void* stream) {
   if (a == nullptr) return noalloc_fail(FT_ERR_INVALID, "null arguments");
-  int rc = check_attention_call(workspace, workspace_bytes, status, a->q.heads, a->k.heads);
+  int rc = check_workspace(workspace, workspace_bytes, status);
+  if (rc == FT_OK) rc = check_heads(a->q.heads, a->k.heads);
   if (rc == FT_OK) rc = check_dtype(a->dtype);
   if (rc == FT_OK) rc = check_scale(a->scale);
   if (rc != FT_OK) return rc;
@@ -543,48 +627,46 @@ int ft_prompt_attention_run(const ft_prompt_attention_args* a, void* workspace, 
   if (a->q_offsets == nullptr) return noalloc_fail(FT_ERR_INVALID, "null q_offsets");
   rc = check_rows(&a->q, "q", a->q.heads);
   if (rc == FT_OK) rc = check_rows(&a->out, "out", a->q.heads);
-  if (rc == FT_OK && a->key_tokens > 0) rc = check_rows(&a->k, "k", a->k.heads);
-  if (rc == FT_OK && a->key_tokens > 0) rc = check_rows(&a->v, "v", a->k.heads);
   if (rc == FT_OK) rc = check_apart(&a->q, "q", a->query_tokens, a->head_dim);
   if (rc == FT_OK) rc = check_apart(&a->out, "out", a->query_tokens, a->head_dim);
-  if (rc == FT_OK && a->key_tokens > 0) rc = check_apart(&a->k, "k", a->key_tokens, a->head_dim);
-  if (rc == FT_OK && a->key_tokens > 0) rc = check_apart(&a->v, "v", a->key_tokens, a->head_dim);
+  if (rc == FT_OK && a->key_tokens > 0) {
+    rc = check_rows(&a->k, "k", a->k.heads);
+    if (rc == FT_OK) rc = check_rows(&a->v, "v", a->k.heads);
+    if (rc == FT_OK) rc = check_apart(&a->k, "k", a->key_tokens, a->head_dim);
+    if (rc == FT_OK) rc = check_apart(&a->v, "v", a->key_tokens, a->head_dim);
+  }
+  int sm_count = 0;
+  if (rc == FT_OK) rc = check_device(&sm_count);
   if (rc != FT_OK) return rc;
+  CUtensorMap maps[2];
+  const ft_rows* kv[2] = {&a->k, &a->v};
+  for (int i = 0; i < 2; ++i) {
+    // without any key nothing is read: the map then only has to be one
+    const ft_rows& rows = a->key_tokens > 0 ? *kv[i] : a->q;
+    const long long dims[3] = {a->head_dim, a->key_tokens > 0 ? a->k.heads : 1, std::max(a->key_tokens, 1)}, strides[2] = {rows.head_stride, rows.token_stride};
+    const int boxes[3] = {64, 1, 128};
+    rc = make_map(&maps[i], a->dtype, rows.data, 3, dims, strides, boxes);
+    if (rc != FT_OK) return rc;
+  }
   ServeAttentionParams p{};
-  p.q = static_cast<const uint16_t*>(a->q.data);
-  p.k = static_cast<const uint16_t*>(a->k.data);
-  p.v = static_cast<const uint16_t*>(a->v.data);
-  p.out = static_cast<uint16_t*>(a->out.data);
   p.lse = a->lse;
-  p.q_token_stride = a->q.token_stride;
-  p.q_head_stride = a->q.head_stride;
-  p.out_token_stride = a->out.token_stride;
-  p.out_head_stride = a->out.head_stride;
-  p.kv_token_stride = a->k.token_stride;
-  p.kv_head_stride = a->k.head_stride;
-  p.v_token_stride = a->v.token_stride;
-  p.v_head_stride = a->v.head_stride;
   p.q_offsets = a->q_offsets;
   p.k_offsets = a->k_offsets != nullptr ? a->k_offsets : a->q_offsets;
   p.batch = a->batch;
   p.query_tokens = a->query_tokens;
   p.key_tokens = a->key_tokens;
-  p.heads = a->q.heads;
   p.kv_heads = a->k.heads;
-  p.group = a->q.heads / a->k.heads;
   p.head_dim = a->head_dim;
   p.causal = a->causal != 0;
-  p.scale_log2 = 1.44269504088896340736f * (a->scale != 0.0f ? a->scale : 1.0f / std::sqrt(static_cast<float>(a->head_dim)));
-  p.status = status;
-  SERVE_CUDA(launch_serve_attention(p, a->dtype, static_cast<cudaStream_t>(stream)));
-  return FT_OK;
+  return attention_run(p, a->q, a->out, maps[0], maps[1], a->dtype, a->scale, workspace, workspace_bytes, status, sm_count, stream);
 }
 
 int ft_tree_attention_run(const ft_kv_cache* cache, const ft_tree_attention_args* a, void* workspace, size_t workspace_bytes, int* status,
                           void* stream) {
   if (a == nullptr) return noalloc_fail(FT_ERR_INVALID, "null arguments");
   int rc = check_cache(cache);
-  if (rc == FT_OK) rc = check_attention_call(workspace, workspace_bytes, status, a->q.heads, cache->kv_heads);
+  if (rc == FT_OK) rc = check_workspace(workspace, workspace_bytes, status);
+  if (rc == FT_OK) rc = check_heads(a->q.heads, cache->kv_heads);
   if (rc == FT_OK) rc = check_scale(a->scale);
   if (rc != FT_OK) return rc;
   if (a->layer < 0 || a->layer >= cache->layers) return noalloc_fail(FT_ERR_INVALID, "layer %d is outside the cache's %d", a->layer, cache->layers);
@@ -602,20 +684,20 @@ int ft_tree_attention_run(const ft_kv_cache* cache, const ft_tree_attention_args
   if (rc == FT_OK) rc = check_rows(&a->out, "out", a->q.heads);
   if (rc == FT_OK) rc = check_apart(&a->q, "q", a->query_tokens, cache->head_dim);
   if (rc == FT_OK) rc = check_apart(&a->out, "out", a->query_tokens, cache->head_dim);
+  int sm_count = 0;
+  if (rc == FT_OK) rc = check_device(&sm_count);
   if (rc != FT_OK) return rc;
+  CUtensorMap maps[2];
+  void* const kv[2] = {cache->k, cache->v};
+  for (int i = 0; i < 2; ++i) {
+    const long long dims[4] = {cache->head_dim, cache->page_size, cache->kv_heads, cache->pages};
+    const long long strides[3] = {cache->token_stride, cache->head_stride, cache->page_stride};
+    const int boxes[4] = {64, std::min(cache->page_size, 128), 1, 1};
+    rc = make_map(&maps[i], cache->dtype, static_cast<const uint16_t*>(kv[i]) + a->layer * cache->layer_stride, 4, dims, strides, boxes);
+    if (rc != FT_OK) return rc;
+  }
   ServeAttentionParams p{};
-  p.q = static_cast<const uint16_t*>(a->q.data);
-  p.k = static_cast<const uint16_t*>(cache->k) + a->layer * cache->layer_stride;
-  p.v = static_cast<const uint16_t*>(cache->v) + a->layer * cache->layer_stride;
-  p.out = static_cast<uint16_t*>(a->out.data);
   p.lse = a->lse;
-  p.q_token_stride = a->q.token_stride;
-  p.q_head_stride = a->q.head_stride;
-  p.out_token_stride = a->out.token_stride;
-  p.out_head_stride = a->out.head_stride;
-  p.kv_token_stride = p.v_token_stride = cache->token_stride;
-  p.kv_head_stride = p.v_head_stride = cache->head_stride;
-  p.page_stride = cache->page_stride;
   p.q_offsets = a->q_offsets;
   p.page_table = a->page_table;
   p.lengths = a->lengths;
@@ -624,19 +706,14 @@ int ft_tree_attention_run(const ft_kv_cache* cache, const ft_tree_attention_args
   p.mask_stride = a->mask_stride;
   p.batch = a->batch;
   p.query_tokens = a->query_tokens;
-  p.heads = a->q.heads;
   p.kv_heads = cache->kv_heads;
-  p.group = a->q.heads / cache->kv_heads;
   p.head_dim = cache->head_dim;
   p.causal = 1;
   p.page_size = cache->page_size;
   p.pages = cache->pages;
   p.table_pages = a->table_pages;
   p.table_stride = a->table_stride;
-  p.scale_log2 = 1.44269504088896340736f * (a->scale != 0.0f ? a->scale : 1.0f / std::sqrt(static_cast<float>(cache->head_dim)));
-  p.status = status;
-  SERVE_CUDA(launch_serve_attention(p, cache->dtype, static_cast<cudaStream_t>(stream)));
-  return FT_OK;
+  return attention_run(p, a->q, a->out, maps[0], maps[1], cache->dtype, a->scale, workspace, workspace_bytes, status, sm_count, stream);
 }
 
 int ft_tree_mask(const int* parents, int nodes, uint32_t* mask, int words) {

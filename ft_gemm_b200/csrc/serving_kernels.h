@@ -1,5 +1,6 @@
 // Internal interface between the serving C-ABI (api_serving.cu) and its kernels.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include "../../include/ft_serving.h"
@@ -48,11 +49,9 @@ cudaError_t launch_accept(const AcceptParams& params, cudaStream_t stream);
 
 // Attention of the queries of each sequence over its keys: packed prompts (page_table == nullptr) or the paged cache.
 struct ServeAttentionParams {
-  const uint16_t *q, *k, *v;
   uint16_t* out;
   float* lse;
-  long long q_token_stride, q_head_stride, out_token_stride, out_head_stride;
-  long long kv_token_stride, kv_head_stride, v_token_stride, v_head_stride, page_stride;
+  long long out_token_stride, out_head_stride;
   const int* q_offsets;
   const int* k_offsets;   // packed prompts
   const int* page_table;  // paged cache
@@ -62,9 +61,16 @@ struct ServeAttentionParams {
   int batch, query_tokens, key_tokens;
   int heads, kv_heads, group, head_dim, causal;
   int page_size, pages, table_pages, table_stride;
+  int min_share;     // key tiles that a CTA takes at least
   float scale_log2;  // log2(e) * scale
+  void* workspace;
   int* status;
 };
-cudaError_t launch_serve_attention(const ServeAttentionParams& params, int dtype, cudaStream_t stream);
+size_t serve_attention_workspace(int sm_count);
+// q: [token][key head][head in group][d], boxes of 128 / group tokens; k, v: [token][key head][d] in boxes of 128 tokens, or
+// [page][key head][token in page][d] in boxes of up to 128 tokens of a page.  split_keys: one row tile per CTA, the two warpgroups
+// take turns on its key tiles.
+cudaError_t launch_serve_attention(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const ServeAttentionParams& params, int dtype,
+                                   bool split_keys, int sm_count, cudaStream_t stream);
 
 }  // namespace ftg
