@@ -4,17 +4,20 @@
 // One persistent CTA per SM takes an equal share of the 128-key tiles of the whole call (serving_schedule.h), so the
 // lengths of the sequences do not matter to the balance, and a long context is split over as many CTAs as there are when
 // there are few rows.  The query heads of a key head are rows of one tile (row = token * group + head in group), which
-// reads K and V once for the group.  Two warpgroups do the softmax, one thread per row, each on scores of its own:
+// reads K and V once for the group.  Two sides A and B work in turn, each on scores and an accumulator of its own:
 //   kSplitKeys = false   two row tiles of 128 rows that share every K and V tile   (many rows)
-//   kSplitKeys = true    one row tile; the warpgroups take the even and the odd key tiles and merge at the end   (few rows)
-// While one warpgroup is in its softmax the tensor core works for the other: scores S = Q K^T into tensor memory, the
+//   kSplitKeys = true    one row tile; the sides take the even and the odd key tiles and merge at the end   (few rows)
+// While one side is in its softmax the tensor core works for the other: scores S = Q K^T into tensor memory, the
 // probabilities go back to tensor memory in 16 bits over the scores they came from, and are the left operand of
-// O += P V.  The exponent's reference follows the running maximum in steps of 2^8 only, so that the accumulator in
-// tensor memory is hardly ever rescaled.
+// O += P V.  A side has two warpgroups, one for each half of the 128 keys, so two threads share a row: one row per thread
+// leaves a scheduler with a single warp per side, whose latencies nothing hides (4 x 4096 tokens, 32 heads of 128: 570 us
+// against KSIDE us).  The exponent's reference follows the running maximum in steps of 2^8 only, so that the accumulator
+// in tensor memory is hardly ever rescaled; the two threads of a row exchange their maxima through shared memory.
 //
 //   warp 0      walks the share: item descriptors for the others, tensor copies of Q, K and V
-//   warp 1      issues the matrix instructions
-//   warps 4-7, 8-11   softmax of A and B, and what leaves the kernel
+//   warp 1      one thread issues the matrix instructions
+//   warp 2      clears what lies behind the last key in the tile of V that holds it
+//   warps 4-7, 8-11, 12-15, 16-19   softmax of (A, first keys), (A, second), (B, first), (B, second), and what leaves the kernel
 //
 // A share that begins or ends inside a row tile leaves its part (unnormalised O, reference and sum of each row) in the
 // workspace; serve_attention_combine_kernel adds the parts up.  Nothing depends on the order in which CTAs run.
@@ -33,23 +36,23 @@ namespace ftg {
 namespace {
 
 constexpr int kRows = 128;  // rows of a tile: the lanes of tensor memory
-constexpr int kThreads = 384;
-// setmaxnreg.inc waits for registers of the CTA's own allotment (384 x 168): the three numbers have to fit together.
-constexpr int kLaunchRegs = 168, kIssueRegs = 72, kSoftmaxRegs = 216;
-static_assert(128 * kIssueRegs + 256 * kSoftmaxRegs <= kThreads * kLaunchRegs, "setmaxnreg.inc would wait for registers the CTA does not own");
-constexpr uint64_t kTimeoutNs = 2000000000ull;
+constexpr int kRoleWarps = 4;                     // in front of the softmax warps
+constexpr int kThreads = (kRoleWarps + 16) * 32;
+// setmaxnreg.inc waits for registers of the CTA's own allotment (640 x 96): the three numbers have to fit together.
+constexpr int kLaunchRegs = 96, kIssueRegs = 56, kSoftmaxRegs = 104;
+static_assert(kThreads == 640 && 128 * kIssueRegs + 512 * kSoftmaxRegs <= kThreads * kLaunchRegs, "setmaxnreg.inc would wait for registers the CTA does not own");
+constexpr uint32_t kTimeoutNs = 2000000000u;
 constexpr float kRescaleStep = 8.0f;  // log2 units
+constexpr int kPolyPairs = 0;         // of eight pairs of exponentials, how many go to the multiply-add pipe
 constexpr int kItems = 4;             // descriptors in flight
 constexpr int kMaxStages = 12;
 constexpr uint32_t kTmemS = 0, kTmemO = 256;  // S of A and B: 128 columns each; O of A and B: kDim each
 
 struct Item {
-  int sequence;
   int token0;      // first query row in q and out
   int tokens;      // queries of this row tile; negative: the walk is over
   int place0;      // place of the first query among the sequence's queries
   int kv_head;
-  int key_row0;    // packed keys: row of the first key
   int prefix, keys, limit;  // limit: no row sees a key at or behind it
   int first, end;  // key tiles of this part
   int slot;        // -1: the whole row tile, straight to the output; otherwise which part in the workspace
@@ -58,28 +61,25 @@ struct Item {
 struct Shared {
   uint64_t kv_full[kMaxStages], kv_empty[kMaxStages];
   uint64_t q_full, q_empty;
-  uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+  uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2];  // p_full: [side][first, second 64 keys]
+  uint64_t tail_wanted, tail_cleared;
   uint64_t item_full[kItems], item_empty[kItems];
   Item items[kItems];
   uint32_t tmem_base;
   int abort_flag;
-  long long scan[kThreads / 32];
-  int start_sequence;
-  long long start_tile;
-  uint64_t state_full;  // kSplitKeys: both warpgroups have written their state
+  uint64_t max_ready[2][4];  // [side][quarter]: both warps of the rows have written the maxima of their keys
+  uint64_t state_full[2];    // [side] (kSplitKeys: the first for both)
+  float row_max[2][2][kRows];     // [side][key half]; written again only when the next scores are there, which follows both reads
+  float2 state[2][2][2][kRows];   // [item parity][side][key half]: {reference, sum} of the rows, in turn for odd and even items
 };
-
-// kSplitKeys, behind Shared: {reference, sum} of each warpgroup's rows, in turn for odd and even items.
-typedef float2 SharedState[2][2][kRows];
 
 template <int kDim, bool kSplitKeys>
 struct Layout {
   static constexpr int kSlabs = kDim / 64;              // 128-byte columns of a row of Q, K or V
   static constexpr int kTileBytes = kSlabs * 128 * 128;
   static constexpr int kQTiles = kSplitKeys ? 1 : 2;
-  static constexpr int kStages = kDim == 64 ? 10 : 5;
-  static constexpr int kBytes = (kQTiles + kStages) * kTileBytes + static_cast<int>(sizeof(Shared)) +
-                                (kSplitKeys ? static_cast<int>(sizeof(SharedState)) : 0) + 1024;
+  static constexpr int kStages = kDim == 64 ? 10 : kSplitKeys ? 5 : 4;
+  static constexpr int kBytes = (kQTiles + kStages) * kTileBytes + static_cast<int>(sizeof(Shared)) + 1024;
   static_assert(kBytes <= 232448 && kStages <= kMaxStages, "shared memory of one CTA");
 };
 
@@ -112,6 +112,27 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// 2^x of two numbers on the multiply-add pipe, for x <= 127: x = i + f with |f| <= 1/2, a polynomial for 2^f, the exponent
+// put together from i.  The special-function unit delivers 16 results per SM and clock, which is what 128 x 128 scores
+// against two products of 128 x 128 x 128 need of it; some of the exponentials here take that load off it.  The
+// polynomial interpolates 2^f at the five Chebyshev nodes of [-1/2, 1/2]: relative error below 3.6e-6.  x below -127 (a masked
+// key: -inf) gives zero; NaN stays NaN.
+__device__ __forceinline__ unsigned long long exp2_poly(float x, float y) {
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(x), "f"(-127.0f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(y), "f"(-127.0f));
+  const unsigned long long v = pack_f32x2(x, y);
+  const unsigned long long whole = add_f32x2(v, pack_f32x2(12582912.0f, 12582912.0f));  // 1.5 * 2^23: rounds to an integer
+  const unsigned long long f = fma_f32x2(add_f32x2(whole, pack_f32x2(-12582912.0f, -12582912.0f)), pack_f32x2(-1.0f, -1.0f), v);
+  unsigned long long r = pack_f32x2(9.666368e-3f, 9.666368e-3f);
+  r = fma_f32x2(r, f, pack_f32x2(5.5921976e-2f, 5.5921976e-2f));
+  r = fma_f32x2(r, f, pack_f32x2(0.2402235f, 0.2402235f));
+  r = fma_f32x2(r, f, pack_f32x2(0.693121f, 0.693121f));
+  r = fma_f32x2(r, f, pack_f32x2(1.0f, 1.0f));
+  float i, j;
+  unpack_f32x2(whole, i, j);
+  const float scale_x = __uint_as_float((__float_as_uint(i) << 23) + 0x3f800000u), scale_y = __uint_as_float((__float_as_uint(j) << 23) + 0x3f800000u);
+  return mul_f32x2(r, pack_f32x2(scale_x, scale_y));
+}
 // Two numbers to 16 bits, the first in the low half.
 template <bool kBf16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
@@ -129,8 +150,26 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
 template <bool kBf16>
 constexpr float kShift = kBf16 ? 0.0f : 7.0f;
 
+// mbar_wait_bounded in few instructions (it stands in some thirty places): gives up after kTimeoutNs, or when another role has.
+__device__ __forceinline__ uint32_t timer_lo() {
+  uint32_t t;
+  asm volatile("mov.u32 %0, %globaltimer_lo;" : "=r"(t));
+  return t;
+}
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint32_t start = timer_lo();
+#pragma unroll 1
+  while (!mbar_try_wait(bar, parity)) {
+    if (*abort_flag != 0 || timer_lo() - start > kTimeoutNs) {
+      *abort_flag = 1;
+      return false;
+    }
+  }
+  return true;
+}
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  return __all_sync(0xffffffffU, mbar_wait_bounded(bar, parity, abort_flag, kTimeoutNs));
+  return __all_sync(0xffffffffU, wait_for(bar, parity, abort_flag));
 }
 
 __device__ __forceinline__ void tma_load_3d(void* smem, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
@@ -143,25 +182,32 @@ __device__ __forceinline__ void tma_load_4d(void* smem, const CUtensorMap* map, 
                "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
                : "memory");
 }
-// D[tmem] (+)= A[tmem] * B[smem], 16-bit operands; A holds two elements per column.
-__device__ __forceinline__ void umma_f16_tmem_a(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+// Shared-memory matrix descriptors (128-byte swizzle, 8 rows of 128 bytes per 1024): the high word is a constant, the low
+// word holds the start address / 16 and, in bits 16 and up, the leading byte offset / 16.  Only the low word is kept in
+// registers: as 64-bit values the descriptors of an unrolled tile take more than a thread has.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+constexpr uint32_t kDescRows = 1u << 16;                    // K-major (Q, K); the offset is not used
+constexpr uint32_t kDescColumns = ((128u * 128u) >> 4) << 16;  // V: 64 elements of a row are contiguous along N, 128 keys further the next 64
+
+// D[tmem] (+)= A[smem] * B[smem]^T, 16-bit operands.
+__device__ __forceinline__ void umma_ss(uint32_t tmem_d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
       : "memory");
 }
-// V as the right operand: 64 elements of a row (one swizzled 128-byte column) are contiguous along N, keys along K.
-// Leading byte offset: from one 64-element column to the next (128 rows of 128 bytes); stride byte offset: 8 keys.
-__device__ __forceinline__ uint64_t make_smem_desc_sw128_mn(uint32_t smem_addr) {
-  uint64_t desc = 0;
-  desc |= static_cast<uint64_t>((smem_addr >> 4) & 0x3fff);
-  desc |= static_cast<uint64_t>((128 * 128) >> 4) << 16;
-  desc |= static_cast<uint64_t>(1024 >> 4) << 32;
-  desc |= static_cast<uint64_t>(1) << 46;
-  desc |= static_cast<uint64_t>(2) << 61;
-  return desc;
+// D[tmem] (+)= A[tmem] * B[smem]; A holds two elements per column.
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
+      : "memory");
 }
 // Instruction descriptor of kind::f16: FP32 accumulator, both operands bf16 (1) or fp16 (0); bit 16: B is N-major.
 template <bool kBf16>
@@ -175,38 +221,59 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
       "r"(r[14]), "r"(r[15])
       : "memory");
 }
-template <int Regs>
-__device__ __forceinline__ void reg_release() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs));
-}
-template <int Regs>
-__device__ __forceinline__ void reg_acquire() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Regs));
-}
-
 // What the call's arrays say about sequence b, cut to what may be read.
 struct Sequence {
   int token0, key_row0;
   SequenceTiles tiles;
 };
-__device__ __forceinline__ Sequence load_sequence(const ServeAttentionParams& p, int b, int tokens_per_item) {
+struct RawSequence {
+  int q_begin, q_end, k_begin, k_end;
+};
+__device__ __forceinline__ RawSequence load_raw(const ServeAttentionParams& p, int b) {
+  RawSequence r;
+  r.q_begin = p.q_offsets[b];
+  r.q_end = p.q_offsets[b + 1];
+  r.k_begin = p.page_table != nullptr ? 0 : p.k_offsets[b];
+  r.k_end = p.page_table != nullptr ? p.lengths[b] : p.k_offsets[b + 1];
+  return r;
+}
+__device__ __forceinline__ Sequence make_sequence(const ServeAttentionParams& p, const RawSequence& r, int tokens_per_item) {
   Sequence s;
-  s.token0 = min(max(p.q_offsets[b], 0), p.query_tokens);
-  const int queries = min(max(p.q_offsets[b + 1], s.token0), p.query_tokens) - s.token0;
+  s.token0 = min(max(r.q_begin, 0), p.query_tokens);
+  const int queries = min(max(r.q_end, s.token0), p.query_tokens) - s.token0;
   int keys, full;
   if (p.page_table != nullptr) {
     s.key_row0 = 0;
-    full = max(p.lengths[b], 0);
+    full = max(r.k_end, 0);
     keys = min(full, p.table_pages * p.page_size);
   } else {
-    s.key_row0 = min(max(p.k_offsets[b], 0), p.key_tokens);
-    keys = full = min(max(p.k_offsets[b + 1], s.key_row0), p.key_tokens) - s.key_row0;
+    s.key_row0 = min(max(r.k_begin, 0), p.key_tokens);
+    keys = full = min(max(r.k_end, s.key_row0), p.key_tokens) - s.key_row0;
   }
   s.tiles = SequenceTiles::make(queries, keys, full, tokens_per_item, p.causal != 0 && p.mask == nullptr);
   return s;
 }
 
-// The queries of warpgroup `half` and the key tiles it works through.
+__device__ __forceinline__ Sequence load_sequence(const ServeAttentionParams& p, int b, int tokens_per_item) {
+  return make_sequence(p, load_raw(p, b), tokens_per_item);
+}
+
+__device__ __forceinline__ Item load_item(const volatile Item& from) {
+  Item i;
+  i.token0 = from.token0;
+  i.tokens = from.tokens;
+  i.place0 = from.place0;
+  i.kv_head = from.kv_head;
+  i.prefix = from.prefix;
+  i.keys = from.keys;
+  i.limit = from.limit;
+  i.first = from.first;
+  i.end = from.end;
+  i.slot = from.slot;
+  return i;
+}
+
+// The queries of side `half` and the key tiles it works through.
 template <bool kSplitKeys>
 struct HalfWork {
   int place0, tokens;  // its first query's place among the item's, how many
@@ -240,9 +307,8 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   uint8_t* smem_q = smem;
   uint8_t* smem_kv = smem + L::kQTiles * L::kTileBytes;
   Shared& sh = *reinterpret_cast<Shared*>(smem_kv + L::kStages * L::kTileBytes);
-  SharedState& state = *reinterpret_cast<SharedState*>(&sh + 1);
   volatile int* abort_flag = &sh.abort_flag;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffU, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;  // warp: in a uniform register
   const int tokens_per_half = kRows / p.group;
   const int tokens_per_item = L::kQTiles * tokens_per_half;
   const bool chain = p.causal != 0 && p.mask == nullptr;
@@ -254,19 +320,22 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     }
     mbar_init(&sh.q_full, 1);
     mbar_init(&sh.q_empty, 1);
-    mbar_init(&sh.state_full, 8);
+    mbar_init(&sh.tail_wanted, 1);
+    mbar_init(&sh.tail_cleared, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.p_full[i][0], 4);
+      mbar_init(&sh.p_full[i][1], 4);
       mbar_init(&sh.o_full[i], 1);
-      mbar_init(&sh.o_empty[i], kSplitKeys ? 8 : 4);
+      mbar_init(&sh.o_empty[i], kSplitKeys ? 16 : 8);
+      mbar_init(&sh.state_full[i], kSplitKeys ? 16 : 8);
+      for (int quarter = 0; quarter < 4; ++quarter) mbar_init(&sh.max_ready[i][quarter], 2);
     }
     for (int i = 0; i < kItems; ++i) {
       mbar_init(&sh.item_full[i], 1);
-      mbar_init(&sh.item_empty[i], 9);
+      mbar_init(&sh.item_empty[i], 18);
     }
     sh.abort_flag = 0;
-    sh.start_sequence = -1;
     fence_barrier_init();
     prefetch_tensormap(&tmap_q);
     prefetch_tensormap(&tmap_k);
@@ -276,81 +345,95 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     tmem_alloc(&sh.tmem_base, 512);
     tmem_relinquish();
   }
-
-  // ---- this CTA's share: the key tiles of all sequences are summed by the whole CTA
-  const int per_thread = (p.batch + kThreads - 1) / kThreads;
-  const int scan_begin = min(static_cast<int>(threadIdx.x) * per_thread, p.batch), scan_end = min(scan_begin + per_thread, p.batch);
-  long long mine = 0;
-  for (int b = scan_begin; b < scan_end; ++b) mine += load_sequence(p, b, tokens_per_item).tiles.tiles_per_head() * p.kv_heads;
-  long long before = mine;  // inclusive prefix within the warp
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const long long other = __shfl_up_sync(0xffffffffU, before, off);
-    if (lane >= off) before += other;
-  }
-  if (lane == 31) sh.scan[warp] = before;
+  // Everything above may run while the kernel in front on the stream still does; nothing below may.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  long long total = 0, front = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) front += sh.scan[w];
-    total += sh.scan[w];
-  }
-  before += front - mine;
-  const long long share = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(p.min_share));
-  const long long share_begin = min(share * blockIdx.x, total), share_end = min(share_begin + share, total);
-  if (share_begin < share_end && before <= share_begin && share_begin < before + mine) {
-    long long at = before;
-    for (int b = scan_begin; b < scan_end; ++b) {
-      const long long here = load_sequence(p, b, tokens_per_item).tiles.tiles_per_head() * p.kv_heads;
-      if (share_begin < at + here) {
-        sh.start_sequence = b;
-        sh.start_tile = share_begin - at;
-        break;
-      }
-      at += here;
-    }
-  }
-  __syncthreads();
   const uint32_t tmem_base = sh.tmem_base;
 
-  if (warp < 4) {
-    reg_release<kIssueRegs>();
+  if (warp < kRoleWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
     if (warp == 0) {
       // ------------------------------------------------------------- the walk, and the tensor copies
+      // this CTA's share: the lanes sum up the sequences' units, each a stretch of sequences
+      Sequence seq = {};
+      int b = 0;
+      long long left, start = 0, share;
+      {
+        const int per_lane = (p.batch + 31) / 32;
+        const int scan_begin = min(lane * per_lane, p.batch), scan_end = min(scan_begin + per_lane, p.batch);
+        long long mine = 0;
+#pragma unroll 1
+        for (int i = scan_begin; i < scan_end; ++i) mine += load_sequence(p, i, tokens_per_item).tiles.units_per_head() * p.kv_heads;
+        long long before = mine;  // inclusive prefix
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const long long other = __shfl_up_sync(0xffffffffU, before, off);
+          if (lane >= off) before += other;
+        }
+        const long long total = __shfl_sync(0xffffffffU, before, 31);
+        before -= mine;
+        share = max(quotient(total + gridDim.x - 1, gridDim.x), static_cast<long long>(p.min_share));
+        const long long share_begin = min(share * blockIdx.x, total);
+        left = min(share_begin + share, total) - share_begin;
+        if (left > 0) {
+          // the lane whose stretch holds the beginning goes through it once more
+          const bool holds = before <= share_begin && share_begin < before + mine;
+          long long at = before;
+          int found = scan_begin;
+          if (holds) {
+#pragma unroll 1
+            for (int i = scan_begin; i + 1 < scan_end; ++i) {
+              const long long here = load_sequence(p, i, tokens_per_item).tiles.units_per_head() * p.kv_heads;
+              if (share_begin < at + here) break;
+              at += here;
+              found = i + 1;
+            }
+          }
+          const int owner = __ffs(__ballot_sync(0xffffffffU, holds)) - 1;
+          b = __shfl_sync(0xffffffffU, found, owner);
+          start = share_begin - __shfl_sync(0xffffffffU, at, owner);
+        }
+      }
       Unfinished unfinished = {};
       int stage = 0, stage_phase = 0, q_phase = 0;
       uint32_t item_index = 0;
       bool ok = true;
-      long long left = share_end - share_begin;
-      int b = sh.start_sequence;
-      Sequence seq = {};
-      int kv_head = 0, row_tile = 0, first = 0, row_tiles_count = 0;
+      int kv_head = 0, row_tile = 0, first = 0;
       if (left > 0) {
         seq = load_sequence(p, b, tokens_per_item);
-        const long long per_head = seq.tiles.tiles_per_head();
-        const long long at = sh.start_tile;
-        kv_head = static_cast<int>(at / per_head);
-        const long long inner = at - kv_head * per_head;
-        int lo = 0, hi = seq.tiles.row_tiles;  // tiles_before(lo) <= inner < tiles_before(hi)
+        const long long per_head = seq.tiles.units_per_head();
+        kv_head = static_cast<int>(quotient(start, per_head));
+        const long long inner = start - kv_head * per_head;
+        int lo = 0, hi = seq.tiles.row_tiles;  // units_before(lo) <= inner < units_before(hi)
+        if (!seq.tiles.ramp) {
+          lo = static_cast<int>(quotient(inner, seq.tiles.units_of(0)));
+          hi = lo + 1;
+        }
         while (hi - lo > 1) {
           const int step = (hi - lo + 31) / 32;
           const int probe = min(lo + lane * step, hi);
-          const int below = __popc(__ballot_sync(0xffffffffU, seq.tiles.tiles_before(probe) <= inner && probe < hi));
+          const int below = __popc(__ballot_sync(0xffffffffU, probe < hi && seq.tiles.units_before(probe) <= inner));
           lo = lo + (below - 1) * step;
           hi = min(lo + step, hi);
         }
         row_tile = lo;
-        first = static_cast<int>(inner - seq.tiles.tiles_before(lo));
+        first = static_cast<int>(inner - seq.tiles.units_before(lo));
+        if (first <= kItemCost) {  // the whole row tile is this CTA's, whatever lies in front of the boundary
+          left += first;
+          first = 0;
+        }
       }
+      RawSequence next = load_raw(p, min(b + 1, p.batch - 1));  // a sequence ahead
       while (ok) {
         const int slot_index = item_index % kItems;
         ok = warp_wait(&sh.item_empty[slot_index], ((item_index / kItems) & 1) ^ 1, abort_flag);
         if (!ok) break;
         Item item = {};
-        if (left <= 0) {
+        const int units = left > 0 ? seq.tiles.units_of(row_tile) : 0;
+        if (left <= 0 || (first == 0 && left <= kItemCost && left < units)) {  // the next CTA takes a row tile that would only begin here
           item.tokens = -1;
           if (lane == 0) {
             sh.items[slot_index] = item;
@@ -358,24 +441,21 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           }
           break;
         }
-        row_tiles_count = seq.tiles.tiles_of(row_tile);
-        const int end = static_cast<int>(min(static_cast<long long>(row_tiles_count), first + left));
-        item.sequence = b;
+        const int end = static_cast<int>(min(static_cast<long long>(units), first + left));
         item.place0 = row_tile * tokens_per_item;
         item.token0 = seq.token0 + item.place0;
         item.tokens = min(seq.tiles.queries - item.place0, tokens_per_item);
         item.kv_head = kv_head;
-        item.key_row0 = seq.key_row0;
         item.prefix = seq.tiles.prefix;
         item.keys = seq.tiles.keys;
         item.limit = seq.tiles.limit(item.place0 + item.tokens);
-        const int real = item.limit <= 0 ? 0 : (item.limit - 1) / kKeyTile + 1;  // a numbered tile may have nothing in it
-        item.first = min(first, real);
-        item.end = min(end, real);
-        item.slot = first == 0 && end == row_tiles_count ? -1 : first > 0 ? 0 : 1;
-        if (first == 0 && end < row_tiles_count) {
+        const int real = item.limit <= 0 ? 0 : (item.limit - 1) / kKeyTile + 1;  // a unit may have no key tile in it
+        item.first = min(max(first - kItemCost, 0), real);
+        item.end = min(max(end - kItemCost, 0), real);
+        item.slot = first == 0 && end == units ? -1 : first > 0 ? 0 : 1;
+        if (first == 0 && end < units) {
           unfinished.valid = 1;
-          unfinished.last_cta = blockIdx.x + static_cast<int>((row_tiles_count - end + share - 1) / share);
+          unfinished.last_cta = blockIdx.x + static_cast<int>(quotient(units - end + share - 1, share));
           unfinished.token0 = item.token0;
           unfinished.tokens = item.tokens;
           unfinished.kv_head = kv_head;
@@ -402,7 +482,17 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
               }
             }
           }
-          auto load = [&](const CUtensorMap* map, int tile) -> bool {
+          const int box = min(p.page_size, kKeyTile);
+          // lane i holds the page of the i-th box of a key tile, asked for a tile ahead; behind the limit nothing is read
+          auto boxes_of = [&](int tile) { return (min(item.limit - tile * kKeyTile, kKeyTile) + box - 1) / box; };
+          auto page_of = [&](int tile) -> int {
+            int page = 0;
+            if (p.page_table != nullptr && tile < item.end && lane < boxes_of(tile)) {
+              page = p.page_table[static_cast<long long>(b) * p.table_stride + (tile * kKeyTile + lane * box) / p.page_size];
+            }
+            return page;
+          };
+          auto load = [&](const CUtensorMap* map, int tile, int page) -> bool {
             if (!warp_wait(&sh.kv_empty[stage], stage_phase ^ 1, abort_flag)) return false;
             uint8_t* to = smem_kv + stage * L::kTileBytes;
             if (p.page_table == nullptr) {
@@ -410,21 +500,19 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 mbar_arrive_expect_tx(&sh.kv_full[stage], L::kTileBytes);
 #pragma unroll
                 for (int sl = 0; sl < L::kSlabs; ++sl) {
-                  tma_load_3d(to + sl * (128 * 128), map, &sh.kv_full[stage], 64 * sl, kv_head, item.key_row0 + tile * kKeyTile);
+                  tma_load_3d(to + sl * (128 * 128), map, &sh.kv_full[stage], 64 * sl, kv_head, seq.key_row0 + tile * kKeyTile);
                 }
               }
             } else {
-              const int box = min(p.page_size, kKeyTile);
-              const int boxes = (min(item.limit - tile * kKeyTile, kKeyTile) + box - 1) / box;  // behind the limit nothing is read
+              const int boxes = boxes_of(tile);
               if (lane == 0) mbar_arrive_expect_tx(&sh.kv_full[stage], boxes * box * L::kSlabs * 128);
               __syncwarp();
               if (lane < boxes) {
-                const int key = tile * kKeyTile + lane * box;
-                int page = p.page_table[static_cast<long long>(b) * p.table_stride + key / p.page_size];
-                if (page < 0 || page > p.pages) page = p.pages;  // outside the tensor: filled with zeros
+                const int place = (tile * kKeyTile + lane * box) & (p.page_size - 1);
+                const int there = page >= 0 && page < p.pages ? page : p.pages;  // outside the tensor: filled with zeros
 #pragma unroll
                 for (int sl = 0; sl < L::kSlabs; ++sl) {
-                  tma_load_4d(to + sl * (128 * 128) + lane * box * 128, map, &sh.kv_full[stage], 64 * sl, key % p.page_size, kv_head, page);
+                  tma_load_4d(to + sl * (128 * 128) + lane * box * 128, map, &sh.kv_full[stage], 64 * sl, place, kv_head, there);
                 }
               }
             }
@@ -434,15 +522,19 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             }
             return true;
           };
-          ok = load(&tmap_k, item.first);
+          int page_v = page_of(item.first), page_k = page_of(item.first + 1), page_ahead = page_of(item.first + 2);
+          ok = load(&tmap_k, item.first, page_v);
           for (int t = item.first; ok && t < item.end; ++t) {
             if (kSplitKeys) {
-              if (t + 1 < item.end) ok = load(&tmap_k, t + 1);
-              if (ok) ok = load(&tmap_v, t);
+              if (t + 1 < item.end) ok = load(&tmap_k, t + 1, page_k);
+              if (ok) ok = load(&tmap_v, t, page_v);
             } else {
-              ok = load(&tmap_v, t);
-              if (ok && t + 1 < item.end) ok = load(&tmap_k, t + 1);
+              ok = load(&tmap_v, t, page_v);
+              if (ok && t + 1 < item.end) ok = load(&tmap_k, t + 1, page_k);
             }
+            page_v = page_k;
+            page_k = page_ahead;
+            page_ahead = page_of(t + 3);
           }
         }
         // the next part
@@ -453,7 +545,9 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           if (++kv_head == p.kv_heads) {
             kv_head = 0;
             do {
-              seq = load_sequence(p, ++b, tokens_per_item);
+              ++b;
+              seq = make_sequence(p, next, tokens_per_item);
+              next = load_raw(p, min(b + 1, p.batch - 1));
             } while (seq.tiles.row_tiles == 0 && b + 1 < p.batch);
           }
         }
@@ -469,213 +563,234 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       }
       if (ok) warp_wait(&sh.q_empty, q_phase ^ 1, abort_flag);
     } else if (warp == 1) {
-      // ------------------------------------------------------------- matrix instructions
-      constexpr uint32_t kIdescS = idesc16<kBf16>(128, false), kIdescO = idesc16<kBf16>(kDim, true);
-      int stage = 0, stage_phase = 0, q_phase = 0;
-      uint32_t p_phase[2] = {0, 0}, o_phase[2] = {0, 0};
-      bool ok = true;
-      const uint32_t q_addr = smem_u32(smem_q), kv_addr = smem_u32(smem_kv);
+      // ------------------------------------------------------------- matrix instructions, all by one thread
+      if (elect_one()) {
+        constexpr uint32_t kIdescS = idesc16<kBf16>(128, false), kIdescO = idesc16<kBf16>(kDim, true);
+        int stage = 0, stage_phase = 0, q_phase = 0, tail_phase = 0;
+        uint32_t p_phase[2] = {0, 0}, o_phase[2] = {0, 0};
+        bool ok = true;
+        const uint32_t q_desc = (smem_u32(smem_q) >> 4) | kDescRows;
+        const uint32_t k_desc = (smem_u32(smem_kv) >> 4) | kDescRows, v_desc = (smem_u32(smem_kv) >> 4) | kDescColumns;
+        auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_for(bar, parity, abort_flag); };
 
-      auto issue_s = [&](int x, int k_stage) {
-        const uint64_t a = make_smem_desc_sw128(q_addr + (kSplitKeys ? 0 : x) * L::kTileBytes), bd = make_smem_desc_sw128(kv_addr + k_stage * L::kTileBytes);
+        auto issue_s = [&](int x, int k_stage) {
+          const uint32_t a = q_desc + (kSplitKeys ? 0 : x) * (L::kTileBytes >> 4), bd = k_desc + k_stage * (L::kTileBytes >> 4);
 #pragma unroll
-        for (int k = 0; k < kDim / 16; ++k) {
-          const int at = (k / 4) * ((128 * 128) >> 4) + (k % 4) * 2;
-          umma_f16(tmem_base + kTmemS + x * 128, a + at, bd + at, kIdescS, k > 0);
-        }
-        umma_commit(&sh.s_full[x]);
-      };
-      auto issue_o = [&](int x, int v_stage, int steps, bool fresh) {
-        const uint64_t bd = make_smem_desc_sw128_mn(kv_addr + v_stage * L::kTileBytes);
-        for (int k = 0; k < steps; ++k) {
-          umma_f16_tmem_a(tmem_base + kTmemO + x * kDim, tmem_base + kTmemS + x * 128 + k * 8, bd + k * (16 * 128 >> 4), kIdescO, !fresh || k > 0);
-        }
-      };
-      auto next_stage = [&]() {
-        if (++stage == L::kStages) {
-          stage = 0;
-          stage_phase ^= 1;
-        }
-      };
-      // V rows behind the last key anyone sees hold whatever memory holds; their probabilities are zero, but zero times
-      // NaN is not, so the instruction stops at the next multiple of 16 keys and the rows up to there are cleared.
-      auto clear_v_tail = [&](int v_stage, int valid) {
-        uint8_t* v = smem_kv + v_stage * L::kTileBytes;
-        const int upto = (valid + 15) / 16 * 16;
-        for (int i = lane; i < (upto - valid) * L::kSlabs * 8; i += 32) {
-          const int row = valid + i / (L::kSlabs * 8), chunk = i % (L::kSlabs * 8);
-          *reinterpret_cast<uint4*>(v + (chunk / 8) * (128 * 128) + row * 128 + (chunk % 8) * 16) = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_shared();
-        __syncwarp();
-      };
+          for (int k = 0; k < kDim / 16; ++k) {
+            const int at = (k / 4) * ((128 * 128) >> 4) + (k % 4) * 2;
+            umma_ss(tmem_base + kTmemS + x * 128, a + at, bd + at, kIdescS, k > 0);
+          }
+          umma_commit(&sh.s_full[x]);
+        };
+        auto next_stage = [&]() {
+          if (++stage == L::kStages) {
+            stage = 0;
+            stage_phase ^= 1;
+          }
+        };
 
-      for (uint32_t index = 0; ok; ++index) {
+        for (uint32_t index = 0; ok; ++index) {
+          const int slot_index = index % kItems;
+          ok = wait(&sh.item_full[slot_index], (index / kItems) & 1);
+          if (!ok) break;
+          const Item item = sh.items[slot_index];
+          mbar_arrive(&sh.item_empty[slot_index]);
+          if (item.tokens < 0) break;
+          const int n = item.end - item.first;
+          if (n <= 0) continue;
+          const int count[2] = {HalfWork<kSplitKeys>(item, 0, tokens_per_half, chain).count, HalfWork<kSplitKeys>(item, 1, tokens_per_half, chain).count};
+          ok = wait(&sh.q_full, q_phase);
+          if (!ok) break;
+          q_phase ^= 1;
+
+          // The tile of V in `v_stage` is there.  Behind the last key that anyone sees it holds whatever memory holds; the
+          // probabilities there are zero, but zero times NaN is not, so the product stops at the next multiple of 16 keys and
+          // warp 2 clears the rows up to it.
+          auto steps_of = [&](int tile) -> int {
+            const int valid = item.limit - tile * kKeyTile;
+            if (valid >= kKeyTile) return 8;
+            if (valid % 16 != 0) {
+              mbar_arrive(&sh.tail_wanted);
+              ok = wait(&sh.tail_cleared, tail_phase);
+              tail_phase ^= 1;
+            }
+            return (valid + 15) / 16;
+          };
+          // O += P V of side x for the key tile in v_stage, its i-th; the probabilities of its first 64 keys lie where their
+          // scores were, those of the others too
+          auto accumulate = [&](int x, int i, int v_stage, int steps) -> bool {
+            if (i == 0) {
+              if (!wait(&sh.o_empty[x], o_phase[x] ^ 1)) return false;
+              o_phase[x] ^= 1;
+            }
+            const uint32_t bd = v_desc + v_stage * (L::kTileBytes >> 4);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (!wait(&sh.p_full[x][h], p_phase[x])) return false;
+              tcgen05_fence_after();
+#pragma unroll
+              for (int k = 4 * h; k < 4 * h + 4; ++k) {
+                if (k < steps) {
+                  umma_ts(tmem_base + kTmemO + x * kDim, tmem_base + kTmemS + x * 128 + h * 64 + (k % 4) * 8, bd + k * (16 * 128 >> 4), kIdescO, i > 0 || k > 0);
+                }
+              }
+            }
+            p_phase[x] ^= 1;
+            if (i + 1 == count[x]) umma_commit(&sh.o_full[x]);
+            return true;
+          };
+
+          if (kSplitKeys) {
+            for (int t = 0; ok && t < min(n, 2); ++t) {
+              ok = wait(&sh.kv_full[stage], stage_phase);
+              if (!ok) break;
+              tcgen05_fence_after();
+              issue_s(t, stage);
+              umma_commit(&sh.kv_empty[stage]);
+              if (t + 1 == n) umma_commit(&sh.q_empty);
+              next_stage();
+            }
+            for (int t = 0; ok && t < n; ++t) {
+              const int x = t & 1;
+              ok = wait(&sh.kv_full[stage], stage_phase);
+              if (!ok) break;
+              const int steps = steps_of(item.first + t);
+              if (ok) ok = accumulate(x, t >> 1, stage, steps);
+              if (!ok) break;
+              umma_commit(&sh.kv_empty[stage]);
+              next_stage();
+              if (t + 2 < n) {
+                ok = wait(&sh.kv_full[stage], stage_phase);
+                if (!ok) break;
+                tcgen05_fence_after();
+                issue_s(x, stage);
+                umma_commit(&sh.kv_empty[stage]);
+                if (t + 3 == n) umma_commit(&sh.q_empty);
+                next_stage();
+              }
+            }
+          } else {
+            ok = wait(&sh.kv_full[stage], stage_phase);
+            if (!ok) break;
+            tcgen05_fence_after();
+            if (count[0] > 0) issue_s(0, stage);
+            if (count[1] > 0) issue_s(1, stage);
+            umma_commit(&sh.kv_empty[stage]);
+            if (n == 1) umma_commit(&sh.q_empty);
+            next_stage();
+            for (int j = 0; ok && j < n; ++j) {
+              const int v_stage = stage;
+              ok = wait(&sh.kv_full[stage], stage_phase);
+              if (!ok) break;
+              next_stage();
+              const int k_stage = stage;
+              if (j + 1 < n) {
+                ok = wait(&sh.kv_full[k_stage], stage_phase);
+                if (!ok) break;
+                next_stage();
+              }
+              const int steps = steps_of(item.first + j);
+              for (int x = 0; ok && x < 2; ++x) {
+                if (j >= count[x]) continue;
+                ok = accumulate(x, j, v_stage, steps);
+                if (ok && j + 1 < count[x]) issue_s(x, k_stage);
+              }
+              if (!ok) break;
+              umma_commit(&sh.kv_empty[v_stage]);
+              if (j + 1 < n) umma_commit(&sh.kv_empty[k_stage]);
+              if (j + 2 == n) umma_commit(&sh.q_empty);
+            }
+          }
+        }
+      }
+    } else if (warp == 2) {
+      // ------------------------------------------------------------- rows of V behind the last key
+      int stage = 0, tail_phase = 0;
+      for (uint32_t index = 0;; ++index) {
         const int slot_index = index % kItems;
-        ok = warp_wait(&sh.item_full[slot_index], (index / kItems) & 1, abort_flag);
-        if (!ok) break;
+        if (!warp_wait(&sh.item_full[slot_index], (index / kItems) & 1, abort_flag)) break;
         const Item item = sh.items[slot_index];
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.item_empty[slot_index]);
         if (item.tokens < 0) break;
         const int n = item.end - item.first;
         if (n <= 0) continue;
-        const int count[2] = {HalfWork<kSplitKeys>(item, 0, tokens_per_half, chain).count, HalfWork<kSplitKeys>(item, 1, tokens_per_half, chain).count};
-        ok = warp_wait(&sh.q_full, q_phase, abort_flag);
-        if (!ok) break;
-        q_phase ^= 1;
-
-        // O += P V of warpgroup x for the key tile in v_stage, its i-th
-        auto accumulate = [&](int x, int i, int v_stage, int steps) -> bool {
-          if (i == 0) {
-            if (!warp_wait(&sh.o_empty[x], o_phase[x] ^ 1, abort_flag)) return false;
-            o_phase[x] ^= 1;
+        stage = (stage + 2 * n) % L::kStages;  // of the 2 n stages that this part goes through, the last holds the tile
+        const int valid = item.limit - (item.end - 1) * kKeyTile;
+        if (valid < kKeyTile && valid % 16 != 0) {
+          if (!warp_wait(&sh.tail_wanted, tail_phase, abort_flag)) break;
+          tail_phase ^= 1;
+          uint8_t* v = smem_kv + (stage + L::kStages - 1) % L::kStages * L::kTileBytes;
+          const int upto = (valid + 15) / 16 * 16;
+          for (int i = lane; i < (upto - valid) * L::kSlabs * 8; i += 32) {
+            const int row = valid + i / (L::kSlabs * 8), chunk = i % (L::kSlabs * 8);
+            *reinterpret_cast<uint4*>(v + (chunk / 8) * (128 * 128) + row * 128 + (chunk % 8) * 16) = make_uint4(0, 0, 0, 0);
           }
-          if (!warp_wait(&sh.p_full[x], p_phase[x], abort_flag)) return false;
-          p_phase[x] ^= 1;
-          tcgen05_fence_after();
-          if (elect_one()) {
-            issue_o(x, v_stage, steps, i == 0);
-            if (i + 1 == count[x]) umma_commit(&sh.o_full[x]);
-          }
+          fence_proxy_async_shared();
           __syncwarp();
-          return true;
-        };
-        auto valid_keys = [&](int tile) { return min(item.limit - tile * kKeyTile, kKeyTile); };
-
-        if (kSplitKeys) {
-          for (int t = 0; ok && t < min(n, 2); ++t) {
-            ok = warp_wait(&sh.kv_full[stage], stage_phase, abort_flag);
-            if (!ok) break;
-            tcgen05_fence_after();
-            if (elect_one()) {
-              issue_s(t, stage);
-              umma_commit(&sh.kv_empty[stage]);
-              if (t + 1 == n) umma_commit(&sh.q_empty);
-            }
-            __syncwarp();
-            next_stage();
-          }
-          for (int t = 0; ok && t < n; ++t) {
-            const int x = t & 1;
-            ok = warp_wait(&sh.kv_full[stage], stage_phase, abort_flag);
-            if (!ok) break;
-            const int valid = valid_keys(item.first + t);
-            if (valid < kKeyTile) clear_v_tail(stage, valid);
-            ok = accumulate(x, t >> 1, stage, (valid + 15) / 16);
-            if (!ok) break;
-            if (elect_one()) umma_commit(&sh.kv_empty[stage]);
-            __syncwarp();
-            next_stage();
-            if (t + 2 < n) {
-              ok = warp_wait(&sh.kv_full[stage], stage_phase, abort_flag);
-              if (!ok) break;
-              tcgen05_fence_after();
-              if (elect_one()) {
-                issue_s(x, stage);
-                umma_commit(&sh.kv_empty[stage]);
-                if (t + 3 == n) umma_commit(&sh.q_empty);
-              }
-              __syncwarp();
-              next_stage();
-            }
-          }
-        } else {
-          ok = warp_wait(&sh.kv_full[stage], stage_phase, abort_flag);
-          if (!ok) break;
-          tcgen05_fence_after();
-          if (elect_one()) {
-            if (count[0] > 0) issue_s(0, stage);
-            if (count[1] > 0) issue_s(1, stage);
-            umma_commit(&sh.kv_empty[stage]);
-            if (n == 1) umma_commit(&sh.q_empty);
-          }
-          __syncwarp();
-          next_stage();
-          for (int j = 0; ok && j < n; ++j) {
-            const int v_stage = stage;
-            ok = warp_wait(&sh.kv_full[stage], stage_phase, abort_flag);
-            if (!ok) break;
-            next_stage();
-            const int k_stage = stage, k_phase = stage_phase;
-            bool have_k = false;
-            if (j + 1 < n) next_stage();
-            const int valid = valid_keys(item.first + j);
-            if (valid < kKeyTile) clear_v_tail(v_stage, valid);
-            for (int x = 0; ok && x < 2; ++x) {
-              if (j >= count[x]) continue;
-              ok = accumulate(x, j, v_stage, (valid + 15) / 16);
-              if (ok && j + 1 < count[x]) {
-                if (!have_k) ok = warp_wait(&sh.kv_full[k_stage], k_phase, abort_flag);
-                have_k = true;
-                if (!ok) break;
-                tcgen05_fence_after();
-                if (elect_one()) issue_s(x, k_stage);
-                __syncwarp();
-              }
-            }
-            if (!ok) break;
-            if (elect_one()) {
-              umma_commit(&sh.kv_empty[v_stage]);
-              if (j + 1 < n) umma_commit(&sh.kv_empty[k_stage]);
-              if (j + 2 == n) umma_commit(&sh.q_empty);
-            }
-            __syncwarp();
-          }
+          if (lane == 0) mbar_arrive(&sh.tail_cleared);
         }
       }
     }
   } else {
-    // --------------------------------------------------------------- softmax: one thread per row
-    reg_acquire<kSoftmaxRegs>();
-    const int x = (warp - 4) >> 2;            // warpgroup A or B
-    const int quarter = warp & 3;             // the lanes of tensor memory this warp can reach
+    // --------------------------------------------------------------- softmax: two threads per row, 64 keys each
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const int group_index = (warp - kRoleWarps) >> 2;
+    const int x = group_index >> 1, c = group_index & 1;  // side, key half
+    const int quarter = warp & 3;                         // the lanes of tensor memory this warp can reach
     const int row = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter) << 21;  // lane index in bits 16 and up, 32 lanes per warp
-    const uint32_t s_addr = tmem_base + lanes + kTmemS + x * 128, o_addr = tmem_base + lanes + kTmemO + x * kDim;
-    const int row_token = row / p.group, row_head = row - row_token * p.group;
-    uint32_t s_phase = 0, o_phase = 0;
+    const uint32_t s_addr = tmem_base + lanes + kTmemS + x * 128 + c * 64;
+    const uint32_t o_addr = tmem_base + lanes + kTmemO + x * kDim + c * (kDim / 2);
+    const int row_token = row / p.group;
+    uint32_t s_phase = 0, o_phase = 0, max_phase = 0;
     bool ok = true;
-    const Parts parts = parts_of(p.workspace, gridDim.x);
 
     for (uint32_t index = 0; ok; ++index) {
       const int slot_index = index % kItems;
       ok = warp_wait(&sh.item_full[slot_index], (index / kItems) & 1, abort_flag);
       if (!ok) break;
-      const Item item = sh.items[slot_index];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.item_empty[slot_index]);
+      // The descriptor stays in shared memory until the row tile is done: the loop over its key tiles needs the registers
+      // (what it spills goes to an L1 cache that shared memory has left next to nothing of).
+      volatile Item& item = sh.items[slot_index];
       if (item.tokens < 0) break;
-      const HalfWork<kSplitKeys> work(item, x, tokens_per_half, chain);
-      const bool real_row = row_token < min(work.tokens, tokens_per_half);
+      int count, plain;  // key tiles of this side; every key below `plain` is seen, with a mask its bits say which of the rest are
+      bool real_row;
+      {
+        const Item copy = load_item(item);
+        const HalfWork<kSplitKeys> work(copy, x, tokens_per_half, chain);
+        count = work.count;
+        real_row = row_token < min(work.tokens, tokens_per_half);
+        plain = !real_row          ? 0
+                : p.mask != nullptr ? min(copy.prefix, copy.keys)
+                : chain             ? min(copy.limit, copy.prefix + copy.place0 + work.place0 + row_token + 1)
+                                    : copy.keys;
+      }
       const bool warp_has_rows = __any_sync(0xffffffffU, real_row);
-      const int place = item.place0 + work.place0 + row_token;  // among the sequence's queries
-      const long long token = item.token0 + work.place0 + row_token;
-      // every key below `plain` is seen; with a mask its bits say which of the rest are
-      const int plain = !real_row ? 0 : p.mask != nullptr ? min(item.prefix, item.keys) : chain ? min(item.limit, item.prefix + place + 1) : item.keys;
-      const uint32_t* mask_row = p.mask != nullptr && real_row ? p.mask + token * p.mask_stride : nullptr;
       const int plain_in_warp = __reduce_min_sync(0xffffffffU, real_row ? plain : 0x7fffffff);
+      int key0 = (item.first + (kSplitKeys ? x : 0)) * kKeyTile + c * 64;
 
       float reference = -INFINITY;  // in units of the exponent, with the type's shift taken off
       float sum = 0.0f;
-      for (int i = 0; i < work.count; ++i) {
-        const int key0 = (item.first + (kSplitKeys ? 2 * i + x : i)) * kKeyTile;
+#pragma unroll 1
+      for (int i = 0; i < count; ++i, key0 += (kSplitKeys ? 2 : 1) * kKeyTile) {
         ok = warp_wait(&sh.s_full[x], s_phase, abort_flag);
         if (!ok) break;
         s_phase ^= 1;
         tcgen05_fence_after();
         if (warp_has_rows) {
-          float s[128];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, s + c * 32);
+          float s[64];
+          tmem_ld_32x32b_x32(s_addr, s);
+          tmem_ld_32x32b_x32(s_addr + 32, s + 32);
           tmem_wait_ld();
-          if (key0 + kKeyTile > plain_in_warp) {
+          if (key0 + 64 > plain_in_warp) {
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
+            for (int w = 0; w < 2; ++w) {
               const int word0 = key0 + w * 32;
               const int seen = min(max(plain - word0, 0), 32);
               uint32_t bits = seen == 32 ? 0xffffffffU : (1u << seen) - 1u;
-              if (mask_row != nullptr && seen < 32) {
+              if (p.mask != nullptr && real_row && seen < 32) {
+                const uint32_t* mask_row = p.mask + static_cast<long long>(item.token0 + (kSplitKeys ? 0 : x * tokens_per_half) + row_token) * p.mask_stride;
                 const int node = word0 - item.prefix;  // of the word's first key; negative before the first drafted token
                 const int word = node >> 5;
                 const uint32_t lo = word >= 0 && word < p.mask_words ? __ldg(mask_row + word) : 0u;
@@ -688,28 +803,36 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
               for (int e = 0; e < 32; ++e) s[w * 32 + e] = (bits >> e) & 1u ? s[w * 32 + e] : -INFINITY;
             }
           }
-          float top_a = s[0], top_b = s[1];
+          float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-          for (int e = 2; e < 126; e += 4) {
-            top_a = max3_f32(top_a, s[e], s[e + 1]);
-            top_b = max3_f32(top_b, s[e + 2], s[e + 3]);
+          for (int e = 4; e < 60; e += 8) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) tops[j] = max3_f32(tops[j], s[e + 2 * j], s[e + 2 * j + 1]);
           }
-          const float top = max3_f32(top_a, top_b, fmaxf(s[126], s[127])) * p.scale_log2 - kShift<kBf16>;
+          tops[0] = max3_f32(tops[0], s[60], s[61]);
+          tops[1] = max3_f32(tops[1], s[62], s[63]);
+          sh.row_max[x][c][row] = fmaxf(max3_f32(tops[0], tops[1], tops[2]), tops[3]) * p.scale_log2 - kShift<kBf16>;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.max_ready[x][quarter]);
+          ok = warp_wait(&sh.max_ready[x][quarter], max_phase, abort_flag);
+          if (!ok) break;
+          max_phase ^= 1;
+          const float top = fmaxf(sh.row_max[x][0][row], sh.row_max[x][1][row]);
           const bool moves = top > reference + kRescaleStep;  // true for the first key that is seen
           if (__any_sync(0xffffffffU, moves)) {
-            const float next = moves ? top : reference;
-            const float shrink = moves ? exp2_approx(reference - next) : 1.0f;  // 0 where nothing was seen before
-            reference = next;
+            // the reference moves for some row: its accumulator and sum shrink
+            const float shrink = moves ? exp2_approx(reference - top) : 1.0f;  // 0 where nothing was seen before
+            if (moves) reference = top;
             sum *= shrink;
             if (i > 0) {
 #pragma unroll 1
-              for (int c = 0; c < kDim / 32; ++c) {
-                float o[32];
-                tmem_ld_32x32b_x32(o_addr + c * 32, o);
+              for (int d = 0; d < kDim / 2; d += 8) {
+                float o[8];
+                tmem_ld_32x32b_x8(o_addr + d, o);
                 tmem_wait_ld();
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] *= shrink;
-                tmem_st_32x32b_x32(o_addr + c * 32, o);
+                for (int e = 0; e < 8; ++e) o[e] *= shrink;
+                tmem_st_32x32b_x8(o_addr + d, o);
               }
             }
           }
@@ -717,22 +840,27 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           const unsigned long long scale2 = pack_f32x2(p.scale_log2, p.scale_log2), base2 = pack_f32x2(-base, -base);
           unsigned long long sum_a = pack_f32x2(sum, 0.0f), sum_b = pack_f32x2(0.0f, 0.0f);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int h = 0; h < 2; ++h) {
             uint32_t packed[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               float lo, hi;
-              unpack_f32x2(fma_f32x2(pack_f32x2(s[c * 32 + 2 * e], s[c * 32 + 2 * e + 1]), scale2, base2), lo, hi);
-              lo = exp2_approx(lo);
-              hi = exp2_approx(hi);
-              if (e & 1) {
-                sum_a = add_f32x2(sum_a, pack_f32x2(lo, hi));
+              unpack_f32x2(fma_f32x2(pack_f32x2(s[h * 32 + 2 * e], s[h * 32 + 2 * e + 1]), scale2, base2), lo, hi);
+              unsigned long long both;
+              if (e % 8 < kPolyPairs) {
+                both = exp2_poly(lo, hi);
               } else {
-                sum_b = add_f32x2(sum_b, pack_f32x2(lo, hi));
+                both = pack_f32x2(exp2_approx(lo), exp2_approx(hi));
               }
+              if (e & 1) {
+                sum_a = add_f32x2(sum_a, both);
+              } else {
+                sum_b = add_f32x2(sum_b, both);
+              }
+              unpack_f32x2(both, lo, hi);
               packed[e] = pack16<kBf16>(lo, hi);
             }
-            tmem_st_32x32b_x16(s_addr + c * 16, packed);
+            tmem_st_32x32b_x16(s_addr + h * 16, packed);
           }
           float lo, hi;
           unpack_f32x2(add_f32x2(sum_a, sum_b), lo, hi);
@@ -741,60 +869,60 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         }
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.p_full[x]);
+        if (lane == 0) mbar_arrive(&sh.p_full[x][c]);
       }
       if (!ok) break;
 
       // ------------------------------------------------------------- what leaves: normalised to the output, or a part
-      float weight_a = 1.0f, weight_b = 0.0f;  // kSplitKeys: of the two warpgroups' sums
-      int count_a = work.count, count_b = 0;
+      // the accumulators are complete once all parts of the probabilities have been used
+      const int n = item.end - item.first;
+      const int count_a = kSplitKeys ? (n + 1) / 2 : count, count_b = kSplitKeys ? n / 2 : 0;
+      if (count_a > 0) ok = warp_wait(&sh.o_full[kSplitKeys ? 0 : x], o_phase & 1, abort_flag);
+      if (ok && count_b > 0) ok = warp_wait(&sh.o_full[1], (o_phase >> 1) & 1, abort_flag);
+      if (!ok) break;
+      if (count_a > 0) o_phase ^= 1;
+      if (count_b > 0) o_phase ^= 2;
+      const int parity = index & 1;
+      sh.state[parity][x][c][row] = make_float2(reference, sum);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.state_full[kSplitKeys ? 0 : x]);
+      ok = warp_wait(&sh.state_full[kSplitKeys ? 0 : x], parity, abort_flag);
+      if (!ok) break;
+      tcgen05_fence_after();
+      float weight_a = 1.0f, weight_b = 0.0f;  // of the two sides' accumulators
       if (kSplitKeys) {
-        // two copies in turn: whoever writes the next but one has seen that all have read this one
-        state[index & 1][x][row] = make_float2(reference, sum);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.state_full);
-        ok = warp_wait(&sh.state_full, index & 1, abort_flag);
-        if (!ok) break;
-        const float2 a = state[index & 1][0][row], bs = state[index & 1][1][row];
-        reference = fmaxf(a.x, bs.x);
+        const float2 a = sh.state[parity][0][0][row], b = sh.state[parity][1][0][row];
+        reference = fmaxf(a.x, b.x);
         const float base = reference == -INFINITY ? 0.0f : reference;
         weight_a = exp2_approx(a.x - base);
-        weight_b = exp2_approx(bs.x - base);
-        sum = a.y * weight_a + bs.y * weight_b;
-        const int n = item.end - item.first;
-        count_a = (n + 1) / 2;
-        count_b = n / 2;
-        // both accumulators are read by both warpgroups, half of the columns each
-        if (count_a > 0) ok = warp_wait(&sh.o_full[0], o_phase & 1, abort_flag);
-        if (ok && count_b > 0) ok = warp_wait(&sh.o_full[1], (o_phase >> 1) & 1, abort_flag);
-        if (!ok) break;
-        if (count_a > 0) o_phase ^= 1;
-        if (count_b > 0) o_phase ^= 2;
-      } else if (work.count > 0) {
-        ok = warp_wait(&sh.o_full[x], o_phase, abort_flag);
-        if (!ok) break;
-        o_phase ^= 1;
+        weight_b = exp2_approx(b.x - base);
+        sum = (a.y + sh.state[parity][0][1][row].y) * weight_a + (b.y + sh.state[parity][1][1][row].y) * weight_b;
+      } else {
+        sum = sh.state[parity][x][0][row].y + sh.state[parity][x][1][row].y;
       }
-      tcgen05_fence_after();
       const int half = kSplitKeys ? 0 : x;
-      const size_t part = (static_cast<size_t>(blockIdx.x) * 2 + max(item.slot, 0)) * 2 + half;
-      const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-      if (kSplitKeys && item.slot < 0) {
+      const int slot = item.slot;
+      const Parts parts = parts_of(p.workspace, gridDim.x);
+      const size_t part = (static_cast<size_t>(blockIdx.x) * 2 + max(slot, 0)) * 2 + half;
+      const int token = item.token0 + (kSplitKeys ? 0 : x * tokens_per_half) + row_token;
+      const int head = item.kv_head * p.group + row - row_token * p.group;
+      if (slot < 0) {
+        const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
         weight_a *= inverse;
         weight_b *= inverse;
-      } else if (item.slot < 0) {
-        weight_a = inverse;
       }
       if (warp_has_rows) {
-        constexpr int kChunk = 32;
-        const int c_begin = kSplitKeys ? x * (kDim / 2) : 0, c_end = kSplitKeys ? c_begin + kDim / 2 : kDim;
+        // the columns of this warpgroup: a half of the head dimension, or (kSplitKeys) a quarter, in chunks
+        constexpr int kColumns = kSplitKeys ? kDim / 4 : kDim / 2, kChunk = 16;
+        const int c_begin = (kSplitKeys ? group_index : c) * kColumns;
         const uint32_t o_a = tmem_base + lanes + kTmemO + half * kDim;
-        uint16_t* out_row = p.out + token * p.out_token_stride + (static_cast<long long>(item.kv_head) * p.group + row_head) * p.out_head_stride;
+        uint16_t* out_row = p.out + token * p.out_token_stride + head * p.out_head_stride;
+        if (!real_row) out_row = nullptr;
 #pragma unroll 1
-        for (int c = c_begin; c < c_end; c += kChunk) {
+        for (int d = c_begin; d < c_begin + kColumns; d += kChunk) {
           float o[kChunk];
           if (count_a > 0) {
-            tmem_ld_32x32b_x32(o_a + c, o);
+            tmem_ld_32x32b_x16(o_a + d, o);
             tmem_wait_ld();
 #pragma unroll
             for (int e = 0; e < kChunk; ++e) o[e] *= weight_a;
@@ -804,40 +932,66 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           }
           if (kSplitKeys && count_b > 0) {
             float o_b[kChunk];
-            tmem_ld_32x32b_x32(o_a + kDim + c, o_b);
+            tmem_ld_32x32b_x16(o_a + kDim + d, o_b);
             tmem_wait_ld();
 #pragma unroll
             for (int e = 0; e < kChunk; ++e) o[e] = fmaf(o_b[e], weight_b, o[e]);
           }
-          if (real_row) {
-            if (item.slot < 0) {
+          if (slot < 0) {
+            // A lane has two pieces of 16 bytes of its row.  Two lanes trade one of theirs each, so that a store
+            // instruction writes whole sectors of 16 rows instead of half sectors of 32.
+            constexpr int kPieces = kChunk / 8;
+            uint32_t piece[kPieces][4];
 #pragma unroll
-              for (int e = 0; e < kChunk; e += 8) {
-                *reinterpret_cast<uint4*>(out_row + c + e) = make_uint4(pack16<kBf16>(o[e], o[e + 1]), pack16<kBf16>(o[e + 2], o[e + 3]),
-                                                                        pack16<kBf16>(o[e + 4], o[e + 5]), pack16<kBf16>(o[e + 6], o[e + 7]));
+            for (int e = 0; e < kChunk / 2; ++e) piece[e / 4][e % 4] = pack16<kBf16>(o[2 * e], o[2 * e + 1]);
+#pragma unroll
+            for (int bit = 1; bit < kPieces; bit <<= 1) {
+              const bool upper = (lane & bit) != 0;
+#pragma unroll
+              for (int i = 0; i < kPieces; ++i) {
+                if (i & bit) continue;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                  const uint32_t got = __shfl_xor_sync(0xffffffffU, upper ? piece[i][w] : piece[i + bit][w], bit);
+                  if (upper) {
+                    piece[i][w] = got;
+                  } else {
+                    piece[i + bit][w] = got;
+                  }
+                }
               }
-            } else {
-              float4* to = parts.o + (part * (kDim / 4) + c / 4) * kRows + row;
-#pragma unroll
-              for (int e = 0; e < kChunk; e += 4) to[e / 4 * kRows] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+              uint16_t* to = reinterpret_cast<uint16_t*>(
+                  __shfl_sync(0xffffffffU, reinterpret_cast<unsigned long long>(out_row), (lane & ~(kPieces - 1)) + i));
+              if (to != nullptr) {
+                *reinterpret_cast<uint4*>(to + d + (lane & (kPieces - 1)) * 8) = make_uint4(piece[i][0], piece[i][1], piece[i][2], piece[i][3]);
+              }
+            }
+          } else if (real_row) {
+            float4* to = parts.o + (part * (kDim / 4) + d / 4) * kRows + row;
+#pragma unroll
+            for (int e = 0; e < kChunk; e += 4) to[e / 4 * kRows] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
         }
-        if (real_row && (!kSplitKeys || x == 0)) {
-          if (item.slot >= 0) {
+        if (real_row && c == 0 && (!kSplitKeys || x == 0)) {
+          if (slot >= 0) {
             parts.state[part * kRows + row] = make_float2(reference, sum);
           } else if (p.lse != nullptr) {
-            p.lse[token * p.heads + item.kv_head * p.group + row_head] = sum == 0.0f ? -INFINITY : (reference + log2f(sum)) * 0.69314718055994531f;
+            p.lse[static_cast<long long>(token) * p.heads + head] =
+                sum == 0.0f ? -INFINITY : (reference + log2f(sum)) * 0.69314718055994531f;
           }
         }
       }
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) {
+        mbar_arrive(&sh.item_empty[slot_index]);
         if (kSplitKeys) {
           if (count_a > 0) mbar_arrive(&sh.o_empty[0]);
           if (count_b > 0) mbar_arrive(&sh.o_empty[1]);
-        } else if (work.count > 0) {
+        } else if (count > 0) {
           mbar_arrive(&sh.o_empty[x]);
         }
       }
@@ -864,6 +1018,8 @@ constexpr int kCombineBlocks = 4, kCombineThreads = 256;
 
 template <int kDim, bool kBf16>
 __global__ void __launch_bounds__(kCombineThreads) serve_attention_combine_kernel(const ServeAttentionParams p, int ctas, int halves) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const Parts parts = parts_of(p.workspace, ctas);
   const int cta = blockIdx.x;
   const Unfinished u = parts.unfinished[cta];
@@ -923,11 +1079,23 @@ static cudaError_t launch_form(const CUtensorMap& q, const CUtensorMap& k, const
     if (err != cudaSuccess) return err;
     configured.fetch_or(bit, std::memory_order_relaxed);
   }
-  serve_attention_kernel<kDim, kBf16, kSplitKeys><<<sm_count, kThreads, L::kBytes, stream>>>(q, k, v, p);
-  err = cudaGetLastError();
+  // Both kernels may start while the one in front of them drains (they wait for its end before they touch memory).
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(sm_count);
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = L::kBytes;
+  config.stream = stream;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  err = cudaLaunchKernelEx(&config, serve_attention_kernel<kDim, kBf16, kSplitKeys>, q, k, v, p);
   if (err != cudaSuccess) return err;
-  serve_attention_combine_kernel<kDim, kBf16><<<dim3(sm_count, kCombineBlocks), kCombineThreads, 0, stream>>>(p, sm_count, L::kQTiles);
-  return cudaGetLastError();
+  config.gridDim = dim3(sm_count, kCombineBlocks);
+  config.blockDim = dim3(kCombineThreads);
+  config.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&config, serve_attention_combine_kernel<kDim, kBf16>, p, sm_count, static_cast<int>(L::kQTiles));
 }
 
 template <int kDim, bool kBf16>
