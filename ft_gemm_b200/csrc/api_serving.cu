@@ -575,6 +575,8 @@ size_t ft_attention_workspace(void) {
   return check_device(&sm_count) == FT_OK ? serve_attention_workspace(sm_count) : 0;
 }
 
+constexpr int kMaxTokens = 1 << 30;  // sums of a few of them stay inside 32 bits
+
 static int check_heads(int heads, int kv_heads) {
   if (kv_heads <= 0 || heads <= 0 || heads % kv_heads != 0 || heads / kv_heads > 128) {
     return noalloc_fail(FT_ERR_INVALID, "query heads (%d) must be 1 to 128 times the key heads (%d)", heads, kv_heads);
@@ -622,7 +624,9 @@ int ft_prompt_attention_run(const ft_prompt_attention_args* a, void* workspace, 
   if (rc == FT_OK) rc = check_scale(a->scale);
   if (rc != FT_OK) return rc;
   if (a->head_dim != 64 && a->head_dim != 128) return noalloc_fail(FT_ERR_INVALID, "head_dim must be 64 or 128 (got %d)", a->head_dim);
-  if (a->batch < 0 || a->query_tokens < 0 || a->key_tokens < 0) return noalloc_fail(FT_ERR_INVALID, "negative batch or token count");
+  if (a->batch < 0 || a->query_tokens < 0 || a->key_tokens < 0 || a->query_tokens > kMaxTokens || a->key_tokens > kMaxTokens) {
+    return noalloc_fail(FT_ERR_INVALID, "negative batch or token count, or more than 2^30 tokens");
+  }
   if (a->batch == 0 || a->query_tokens == 0) return FT_OK;
   if (a->q_offsets == nullptr) return noalloc_fail(FT_ERR_INVALID, "null q_offsets");
   rc = check_rows(&a->q, "q", a->q.heads);
@@ -670,9 +674,11 @@ int ft_tree_attention_run(const ft_kv_cache* cache, const ft_tree_attention_args
   if (rc == FT_OK) rc = check_scale(a->scale);
   if (rc != FT_OK) return rc;
   if (a->layer < 0 || a->layer >= cache->layers) return noalloc_fail(FT_ERR_INVALID, "layer %d is outside the cache's %d", a->layer, cache->layers);
-  if (a->batch < 0 || a->query_tokens < 0) return noalloc_fail(FT_ERR_INVALID, "negative batch or token count");
-  if (a->table_pages <= 0 || a->table_stride < a->table_pages || a->table_pages > INT32_MAX / cache->page_size) {
-    return noalloc_fail(FT_ERR_INVALID, "the page table needs columns (below 2^31 tokens) and a stride that holds them (got %d, %d)", a->table_pages,
+  if (a->batch < 0 || a->query_tokens < 0 || a->query_tokens > kMaxTokens) {
+    return noalloc_fail(FT_ERR_INVALID, "negative batch or token count, or more than 2^30 tokens");
+  }
+  if (a->table_pages <= 0 || a->table_stride < a->table_pages || a->table_pages > kMaxTokens / cache->page_size) {
+    return noalloc_fail(FT_ERR_INVALID, "the page table needs columns (at most 2^30 tokens) and a stride that holds them (got %d, %d)", a->table_pages,
                         a->table_stride);
   }
   if (a->mask != nullptr && (a->mask_words <= 0 || a->mask_stride < a->mask_words)) {

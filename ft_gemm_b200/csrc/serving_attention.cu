@@ -360,13 +360,17 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       // this CTA's share: the lanes sum up the sequences' units, each a stretch of sequences
       Sequence seq = {};
       int b = 0;
-      long long left, start = 0, share;
+      long long left, start = 0, share, per_head = 1;
       {
         const int per_lane = (p.batch + 31) / 32;
         const int scan_begin = min(lane * per_lane, p.batch), scan_end = min(scan_begin + per_lane, p.batch);
-        long long mine = 0;
+        long long mine = 0, units = 0;  // units: of one head of the last sequence looked at
 #pragma unroll 1
-        for (int i = scan_begin; i < scan_end; ++i) mine += load_sequence(p, i, tokens_per_item).tiles.units_per_head() * p.kv_heads;
+        for (int i = scan_begin; i < scan_end; ++i) {
+          seq = load_sequence(p, i, tokens_per_item);
+          units = seq.tiles.units_per_head();
+          mine += units * p.kv_heads;
+        }
         long long before = mine;  // inclusive prefix
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -379,22 +383,27 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         const long long share_begin = min(share * blockIdx.x, total);
         left = min(share_begin + share, total) - share_begin;
         if (left > 0) {
-          // the lane whose stretch holds the beginning goes through it once more
+          // the lane whose stretch holds the beginning goes through it once more, unless it is one sequence
           const bool holds = before <= share_begin && share_begin < before + mine;
           long long at = before;
           int found = scan_begin;
-          if (holds) {
+          if (holds && per_lane > 1) {
 #pragma unroll 1
-            for (int i = scan_begin; i + 1 < scan_end; ++i) {
-              const long long here = load_sequence(p, i, tokens_per_item).tiles.units_per_head() * p.kv_heads;
-              if (share_begin < at + here) break;
-              at += here;
-              found = i + 1;
+            for (; found < scan_end; ++found) {
+              seq = load_sequence(p, found, tokens_per_item);
+              units = seq.tiles.units_per_head();
+              if (share_begin < at + units * p.kv_heads) break;
+              at += units * p.kv_heads;
             }
           }
           const int owner = __ffs(__ballot_sync(0xffffffffU, holds)) - 1;
           b = __shfl_sync(0xffffffffU, found, owner);
           start = share_begin - __shfl_sync(0xffffffffU, at, owner);
+          per_head = __shfl_sync(0xffffffffU, units, owner);
+          seq.token0 = __shfl_sync(0xffffffffU, seq.token0, owner);
+          seq.key_row0 = __shfl_sync(0xffffffffU, seq.key_row0, owner);
+          seq.tiles = SequenceTiles::make(__shfl_sync(0xffffffffU, seq.tiles.queries, owner), __shfl_sync(0xffffffffU, seq.tiles.keys, owner),
+                                          __shfl_sync(0xffffffffU, seq.tiles.prefix + seq.tiles.queries, owner), tokens_per_item, chain);
         }
       }
       Unfinished unfinished = {};
@@ -403,24 +412,26 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       bool ok = true;
       int kv_head = 0, row_tile = 0, first = 0;
       if (left > 0) {
-        seq = load_sequence(p, b, tokens_per_item);
-        const long long per_head = seq.tiles.units_per_head();
         kv_head = static_cast<int>(quotient(start, per_head));
         const long long inner = start - kv_head * per_head;
-        int lo = 0, hi = seq.tiles.row_tiles;  // units_before(lo) <= inner < units_before(hi)
-        if (!seq.tiles.ramp) {
+        int lo = 0;
+        long long in_front = 0;  // units_before(lo) <= inner
+        if (seq.tiles.ramp) {
+          for (int hi = seq.tiles.row_tiles; hi - lo > 1;) {
+            const int step = (hi - lo + 31) / 32;
+            const int probe = min(lo + lane * step, hi);
+            const long long units = seq.tiles.units_before(probe);
+            const int last = __popc(__ballot_sync(0xffffffffU, probe < hi && units <= inner)) - 1;
+            in_front = __shfl_sync(0xffffffffU, units, last);
+            lo = lo + last * step;
+            hi = min(lo + step, hi);
+          }
+        } else {
           lo = static_cast<int>(quotient(inner, seq.tiles.units_of(0)));
-          hi = lo + 1;
-        }
-        while (hi - lo > 1) {
-          const int step = (hi - lo + 31) / 32;
-          const int probe = min(lo + lane * step, hi);
-          const int below = __popc(__ballot_sync(0xffffffffU, probe < hi && seq.tiles.units_before(probe) <= inner));
-          lo = lo + (below - 1) * step;
-          hi = min(lo + step, hi);
+          in_front = static_cast<long long>(lo) * seq.tiles.units_of(0);
         }
         row_tile = lo;
-        first = static_cast<int>(inner - seq.tiles.units_before(lo));
+        first = static_cast<int>(inner - in_front);
         if (first <= kItemCost) {  // the whole row tile is this CTA's, whatever lies in front of the boundary
           left += first;
           first = 0;
@@ -1036,21 +1047,20 @@ __global__ void __launch_bounds__(kCombineThreads) serve_attention_combine_kerne
     if (row_token >= tokens_per_half || half * tokens_per_half + row_token >= u.tokens) continue;
     // the first part lies in slot 1 of its CTA, the others in slot 0
     auto part_at = [&](int c) { return (static_cast<size_t>(c) * 2 + (c == cta ? 1 : 0)) * 2 + half; };
-    float reference = -INFINITY;
-    for (int c = cta; c <= u.last_cta; ++c) reference = fmaxf(reference, parts.state[part_at(c) * kRows + row].x);
-    const float base = reference == -INFINITY ? 0.0f : reference;
-    float sum = 0.0f;
+    float reference = -INFINITY, sum = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
     for (int c = cta; c <= u.last_cta; ++c) {
       const float2 state = parts.state[part_at(c) * kRows + row];
       const float4 add = parts.o[(part_at(c) * (kDim / 4) + columns) * kRows + row];
-      const float weight = exp2_approx(state.x - base);
-      sum = fmaf(state.y, weight, sum);
-      o.x = fmaf(add.x, weight, o.x);
-      o.y = fmaf(add.y, weight, o.y);
-      o.z = fmaf(add.z, weight, o.z);
-      o.w = fmaf(add.w, weight, o.w);
+      const float next = fmaxf(reference, state.x), base = next == -INFINITY ? 0.0f : next;
+      const float shrink = exp2_approx(reference - base), weight = exp2_approx(state.x - base);
+      reference = next;
+      sum = fmaf(state.y, weight, sum * shrink);
+      o.x = fmaf(add.x, weight, o.x * shrink);
+      o.y = fmaf(add.y, weight, o.y * shrink);
+      o.z = fmaf(add.z, weight, o.z * shrink);
+      o.w = fmaf(add.w, weight, o.w * shrink);
     }
     const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
     const long long token = u.token0 + half * tokens_per_half + row_token;

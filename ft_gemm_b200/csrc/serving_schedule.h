@@ -9,7 +9,6 @@
 #pragma once
 #include <stdint.h>
 
-// FT_HD_CALL: a function of its own in device code, where these steps stand beside loops that want the instruction cache.
 #ifdef __CUDACC__
 #define FT_HD __host__ __device__ __forceinline__
 #define FT_HD_CALL static __host__ __device__ __noinline__
@@ -23,36 +22,29 @@ namespace ftg {
 constexpr int kKeyTile = 128;
 constexpr int kItemCost = 2;
 
+FT_HD_CALL long long wide_quotient(long long a, long long b) { return a / b; }
 // 64-bit numbers that nearly always fit into 32 bits, where a division is several times cheaper
-FT_HD_CALL long long quotient(long long a, long long b) {
+FT_HD long long quotient(long long a, long long b) {
   if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
-  return a / b;
+  return wide_quotient(a, b);
 }
 
-// sum over i in [0, n) of floor((a i + b) / m) for a, b >= 0, m > 0, in O(log) steps (the Euclid-like recursion on lattice
-// points under a line)
-FT_HD_CALL long long floor_sum(long long n, long long m, long long a, long long b) {
-  long long total = 0;
-  while (n > 0) {
-    if (a >= m) {
-      const long long whole = quotient(a, m);
-      total += n * (n - 1) / 2 * whole;
-      a -= whole * m;
-    }
-    if (b >= m) {
-      const long long whole = quotient(b, m);
-      total += n * whole;
-      b -= whole * m;
-    }
-    const long long top = a * n + b;
-    if (top < m) break;
-    n = quotient(top, m);
-    b = top - n * m;
-    const long long t = m;
-    m = a;
-    a = t;
+// sum over i in [0, n) of floor((a i + b) / 128) for a, b >= 0.  The steps repeat every 128 / gcd(a, 128) terms with an
+// increment of a / gcd(a, 128): one period is added up term by term (at most 128 of them; at most 4 for the usual head groups), the
+// rest follows.
+FT_HD long long floor_sum(int n, int a, int b) {
+  if (n <= 0) return 0;
+  int shift = 0;  // period = 2^shift
+  while (((a << shift) & (kKeyTile - 1)) != 0) ++shift;
+  const int period = 1 << shift, step = (a << shift) / kKeyTile, periods = n >> shift, rest = n & (period - 1);
+  long long one = 0, head = 0;  // a whole period, and its first `rest` terms
+  int at = b;
+  for (int i = 0; i < period; ++i, at += a) {
+    if (i == rest) head = one;
+    one += at / kKeyTile;
   }
-  return total;
+  return periods * one + static_cast<long long>(step) * period * (static_cast<long long>(periods) * (periods - 1) / 2) + head +
+         static_cast<long long>(rest) * periods * step;
 }
 
 struct SequenceTiles {
@@ -88,21 +80,19 @@ struct SequenceTiles {
     return tiles(limit(end < queries ? static_cast<int>(end) : queries)) + kItemCost;
   }
   // units of the row tiles in front of r, r in [0, row_tiles]
-  FT_HD long long units_before(int r) const { return units_before_of(*this, r); }
-  FT_HD long long units_per_head() const { return row_tiles == 0 ? 0 : units_before(row_tiles); }
-  FT_HD_CALL long long units_before_of(const SequenceTiles& t, int r) {
-    if (!t.ramp) return static_cast<long long>(r) * (tiles(t.keys) + kItemCost);
-    const int inner = r < t.row_tiles ? r : t.row_tiles - 1;  // the last row tile ends with the queries, not on the line
-    long long empty = 0;                                  // row tiles that see nothing
-    if (t.prefix < 0) {
-      empty = quotient(t.tokens_per_item - t.prefix, t.tokens_per_item) - 1;
+  FT_HD long long units_before(int r) const {
+    if (!ramp) return static_cast<long long>(r) * (tiles(keys) + kItemCost);
+    const int inner = r < row_tiles ? r : row_tiles - 1;  // the last row tile ends with the queries, not on the line
+    int empty = 0;                                        // row tiles that see nothing
+    if (prefix < 0) {
+      empty = -prefix / tokens_per_item;
       empty = empty > inner ? inner : empty;
     }
-    long long total = static_cast<long long>(inner) * kItemCost + empty +
-                      floor_sum(inner - empty, kKeyTile, t.tokens_per_item, static_cast<long long>(t.tokens_per_item) * (empty + 1) + t.prefix + kKeyTile - 1);
-    if (r == t.row_tiles && t.row_tiles > 0) total += t.units_of(t.row_tiles - 1);
+    long long total = static_cast<long long>(inner) * kItemCost + empty + floor_sum(inner - empty, tokens_per_item, tokens_per_item * (empty + 1) + prefix + kKeyTile - 1);
+    if (r == row_tiles && row_tiles > 0) total += units_of(row_tiles - 1);
     return total;
   }
+  FT_HD long long units_per_head() const { return row_tiles == 0 ? 0 : units_before(row_tiles); }
 };
 
 }  // namespace ftg
