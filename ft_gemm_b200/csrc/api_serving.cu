@@ -605,6 +605,7 @@ static int attention_run(ServeAttentionParams& p, const ft_rows& q, const ft_row
   p.out_head_stride = out.head_stride;
   p.heads = q.heads;
   p.group = q.heads / p.kv_heads;
+  p.tokens_per_tile = 128 / p.group;
   p.scale_log2 = 1.44269504088896340736f * (scale != 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(p.head_dim)));
   p.min_share = 1;
   p.workspace = workspace;

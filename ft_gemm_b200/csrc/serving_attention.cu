@@ -17,7 +17,7 @@
 //   warp 0      walks the share: item descriptors for the others, tensor copies of Q, K and V
 //   warp 1      one thread issues the matrix instructions
 //   warp 2      clears what lies behind the last key in the tile of V that holds it
-//   warps 4-7, 8-11, 12-15, 16-19   softmax of (A, first keys), (A, second), (B, first), (B, second), and what leaves the kernel
+//   warps 3-6, 7-10, 11-14, 15-18   softmax of (A, first keys), (A, second), (B, first), (B, second), and what leaves the kernel
 //
 // A share that begins or ends inside a row tile leaves its part (unnormalised O, reference and sum of each row) in the
 // workspace; serve_attention_combine_kernel adds the parts up.  Nothing depends on the order in which CTAs run.
@@ -36,14 +36,10 @@ namespace ftg {
 namespace {
 
 constexpr int kRows = 128;  // rows of a tile: the lanes of tensor memory
-constexpr int kRoleWarps = 4;                     // in front of the softmax warps
-constexpr int kThreads = (kRoleWarps + 16) * 32;
-// setmaxnreg.inc waits for registers of the CTA's own allotment (640 x 96): the three numbers have to fit together.
-constexpr int kLaunchRegs = 96, kIssueRegs = 56, kSoftmaxRegs = 104;
-static_assert(kThreads == 640 && 128 * kIssueRegs + 512 * kSoftmaxRegs <= kThreads * kLaunchRegs, "setmaxnreg.inc would wait for registers the CTA does not own");
+constexpr int kRoleWarps = 3;                     // in front of the softmax warps
+constexpr int kThreads = (kRoleWarps + 16) * 32;  // 96 registers each: nothing spills in the loops, and spills go to an L1 cache that shared memory has left little of
 constexpr uint32_t kTimeoutNs = 2000000000u;
 constexpr float kRescaleStep = 8.0f;  // log2 units
-constexpr int kPolyPairs = 0;         // of eight pairs of exponentials, how many go to the multiply-add pipe
 constexpr int kItems = 4;             // descriptors in flight
 constexpr int kMaxStages = 12;
 constexpr uint32_t kTmemS = 0, kTmemO = 256;  // S of A and B: 128 columns each; O of A and B: kDim each
@@ -111,27 +107,6 @@ __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-// 2^x of two numbers on the multiply-add pipe, for x <= 127: x = i + f with |f| <= 1/2, a polynomial for 2^f, the exponent
-// put together from i.  The special-function unit delivers 16 results per SM and clock, which is what 128 x 128 scores
-// against two products of 128 x 128 x 128 need of it; some of the exponentials here take that load off it.  The
-// polynomial interpolates 2^f at the five Chebyshev nodes of [-1/2, 1/2]: relative error below 3.6e-6.  x below -127 (a masked
-// key: -inf) gives zero; NaN stays NaN.
-__device__ __forceinline__ unsigned long long exp2_poly(float x, float y) {
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(x), "f"(-127.0f));
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(y), "f"(-127.0f));
-  const unsigned long long v = pack_f32x2(x, y);
-  const unsigned long long whole = add_f32x2(v, pack_f32x2(12582912.0f, 12582912.0f));  // 1.5 * 2^23: rounds to an integer
-  const unsigned long long f = fma_f32x2(add_f32x2(whole, pack_f32x2(-12582912.0f, -12582912.0f)), pack_f32x2(-1.0f, -1.0f), v);
-  unsigned long long r = pack_f32x2(9.666368e-3f, 9.666368e-3f);
-  r = fma_f32x2(r, f, pack_f32x2(5.5921976e-2f, 5.5921976e-2f));
-  r = fma_f32x2(r, f, pack_f32x2(0.2402235f, 0.2402235f));
-  r = fma_f32x2(r, f, pack_f32x2(0.693121f, 0.693121f));
-  r = fma_f32x2(r, f, pack_f32x2(1.0f, 1.0f));
-  float i, j;
-  unpack_f32x2(whole, i, j);
-  const float scale_x = __uint_as_float((__float_as_uint(i) << 23) + 0x3f800000u), scale_y = __uint_as_float((__float_as_uint(j) << 23) + 0x3f800000u);
-  return mul_f32x2(r, pack_f32x2(scale_x, scale_y));
 }
 // Two numbers to 16 bits, the first in the low half.
 template <bool kBf16>
@@ -309,7 +284,7 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   Shared& sh = *reinterpret_cast<Shared*>(smem_kv + L::kStages * L::kTileBytes);
   volatile int* abort_flag = &sh.abort_flag;
   const int warp = __shfl_sync(0xffffffffU, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;  // warp: in a uniform register
-  const int tokens_per_half = kRows / p.group;
+  const int tokens_per_half = p.tokens_per_tile;
   const int tokens_per_item = L::kQTiles * tokens_per_half;
   const bool chain = p.causal != 0 && p.mask == nullptr;
 
@@ -348,64 +323,75 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   // Everything above may run while the kernel in front on the stream still does; nothing below may.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // ---- this CTA's share (warp 0): the lanes sum up the sequences' units, a stretch of sequences each
+  Sequence seq = {};
+  int first_sequence = 0;
+  long long left = 0, start = 0, share = 0, per_head = 1;  // units of the share; of it, in front in its sequence; per CTA; per key head
+  if (warp == 0) {
+    const int per_lane = (p.batch + 31) / 32;
+    const int scan_begin = min(lane * per_lane, p.batch), scan_end = min(scan_begin + per_lane, p.batch);
+    long long mine = 0, before = 0, share_begin = 0, at = 0;
+    bool holds = false;
+    int found = scan_begin;
+    // first the sums; then the lane whose stretch holds the beginning goes through it once more, unless it is one sequence
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll 1
+      for (int i = scan_begin; i < scan_end; ++i) {
+        seq = load_sequence(p, i, tokens_per_item);
+        per_head = seq.tiles.units_per_head();
+        const long long units = per_head * p.kv_heads;
+        if (pass == 0) {
+          mine += units;
+        } else {
+          found = i;
+          if (share_begin < at + units) break;
+          at += units;
+        }
+      }
+      if (pass == 1) break;
+      before = mine;  // inclusive prefix
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const long long other = __shfl_up_sync(0xffffffffU, before, off);
+        if (lane >= off) before += other;
+      }
+      const long long total = __shfl_sync(0xffffffffU, before, 31);
+      before -= mine;
+      share = max(quotient(total + gridDim.x - 1, gridDim.x), static_cast<long long>(p.min_share));
+      share_begin = min(share * blockIdx.x, total);
+      left = min(share_begin + share, total) - share_begin;
+      holds = left > 0 && before <= share_begin && share_begin < before + mine;
+      at = before;
+      if (!holds || per_lane == 1) break;
+    }
+    __syncwarp();
+    if (left > 0) {
+      const int owner = __ffs(__ballot_sync(0xffffffffU, holds)) - 1;
+      first_sequence = __shfl_sync(0xffffffffU, found, owner);
+      start = share_begin - __shfl_sync(0xffffffffU, at, owner);
+      per_head = __shfl_sync(0xffffffffU, per_head, owner);
+      seq.token0 = __shfl_sync(0xffffffffU, seq.token0, owner);
+      seq.key_row0 = __shfl_sync(0xffffffffU, seq.key_row0, owner);
+      seq.tiles.queries = __shfl_sync(0xffffffffU, seq.tiles.queries, owner);
+      seq.tiles.keys = __shfl_sync(0xffffffffU, seq.tiles.keys, owner);
+      seq.tiles.prefix = __shfl_sync(0xffffffffU, seq.tiles.prefix, owner);
+      seq.tiles.row_tiles = __shfl_sync(0xffffffffU, seq.tiles.row_tiles, owner);
+      seq.tiles.tokens_per_item = tokens_per_item;
+      seq.tiles.chain = chain;
+      seq.tiles.ramp = __shfl_sync(0xffffffffU, seq.tiles.ramp ? 1 : 0, owner) != 0;
+    }
+  }
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem_base = sh.tmem_base;
 
   if (warp < kRoleWarps) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
     if (warp == 0) {
       // ------------------------------------------------------------- the walk, and the tensor copies
-      // this CTA's share: the lanes sum up the sequences' units, each a stretch of sequences
-      Sequence seq = {};
-      int b = 0;
-      long long left, start = 0, share, per_head = 1;
-      {
-        const int per_lane = (p.batch + 31) / 32;
-        const int scan_begin = min(lane * per_lane, p.batch), scan_end = min(scan_begin + per_lane, p.batch);
-        long long mine = 0, units = 0;  // units: of one head of the last sequence looked at
-#pragma unroll 1
-        for (int i = scan_begin; i < scan_end; ++i) {
-          seq = load_sequence(p, i, tokens_per_item);
-          units = seq.tiles.units_per_head();
-          mine += units * p.kv_heads;
-        }
-        long long before = mine;  // inclusive prefix
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-          const long long other = __shfl_up_sync(0xffffffffU, before, off);
-          if (lane >= off) before += other;
-        }
-        const long long total = __shfl_sync(0xffffffffU, before, 31);
-        before -= mine;
-        share = max(quotient(total + gridDim.x - 1, gridDim.x), static_cast<long long>(p.min_share));
-        const long long share_begin = min(share * blockIdx.x, total);
-        left = min(share_begin + share, total) - share_begin;
-        if (left > 0) {
-          // the lane whose stretch holds the beginning goes through it once more, unless it is one sequence
-          const bool holds = before <= share_begin && share_begin < before + mine;
-          long long at = before;
-          int found = scan_begin;
-          if (holds && per_lane > 1) {
-#pragma unroll 1
-            for (; found < scan_end; ++found) {
-              seq = load_sequence(p, found, tokens_per_item);
-              units = seq.tiles.units_per_head();
-              if (share_begin < at + units * p.kv_heads) break;
-              at += units * p.kv_heads;
-            }
-          }
-          const int owner = __ffs(__ballot_sync(0xffffffffU, holds)) - 1;
-          b = __shfl_sync(0xffffffffU, found, owner);
-          start = share_begin - __shfl_sync(0xffffffffU, at, owner);
-          per_head = __shfl_sync(0xffffffffU, units, owner);
-          seq.token0 = __shfl_sync(0xffffffffU, seq.token0, owner);
-          seq.key_row0 = __shfl_sync(0xffffffffU, seq.key_row0, owner);
-          seq.tiles = SequenceTiles::make(__shfl_sync(0xffffffffU, seq.tiles.queries, owner), __shfl_sync(0xffffffffU, seq.tiles.keys, owner),
-                                          __shfl_sync(0xffffffffU, seq.tiles.prefix + seq.tiles.queries, owner), tokens_per_item, chain);
-        }
-      }
+      int b = first_sequence;
       Unfinished unfinished = {};
       int stage = 0, stage_phase = 0, q_phase = 0;
       uint32_t item_index = 0;
@@ -714,7 +700,7 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           }
         }
       }
-    } else if (warp == 2) {
+    } else {
       // ------------------------------------------------------------- rows of V behind the last key
       int stage = 0, tail_phase = 0;
       for (uint32_t index = 0;; ++index) {
@@ -745,7 +731,6 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     }
   } else {
     // --------------------------------------------------------------- softmax: two threads per row, 64 keys each
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int group_index = (warp - kRoleWarps) >> 2;
     const int x = group_index >> 1, c = group_index & 1;  // side, key half
     const int quarter = warp & 3;                         // the lanes of tensor memory this warp can reach
@@ -857,18 +842,13 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             for (int e = 0; e < 16; ++e) {
               float lo, hi;
               unpack_f32x2(fma_f32x2(pack_f32x2(s[h * 32 + 2 * e], s[h * 32 + 2 * e + 1]), scale2, base2), lo, hi);
-              unsigned long long both;
-              if (e % 8 < kPolyPairs) {
-                both = exp2_poly(lo, hi);
-              } else {
-                both = pack_f32x2(exp2_approx(lo), exp2_approx(hi));
-              }
+              lo = exp2_approx(lo);
+              hi = exp2_approx(hi);
               if (e & 1) {
-                sum_a = add_f32x2(sum_a, both);
+                sum_a = add_f32x2(sum_a, pack_f32x2(lo, hi));
               } else {
-                sum_b = add_f32x2(sum_b, both);
+                sum_b = add_f32x2(sum_b, pack_f32x2(lo, hi));
               }
-              unpack_f32x2(both, lo, hi);
               packed[e] = pack16<kBf16>(lo, hi);
             }
             tmem_st_32x32b_x16(s_addr + h * 16, packed);
@@ -1025,7 +1005,7 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
 
 // Adds up the parts of the row tiles that were split over CTAs: block (c, y) takes the row tile that begins in CTA c and
 // does not end there.  A thread has four columns of one row; lanes run over rows first, as the parts are laid out.
-constexpr int kCombineBlocks = 4, kCombineThreads = 256;
+constexpr int kCombineBlocks = 8, kCombineThreads = 256;
 
 template <int kDim, bool kBf16>
 __global__ void __launch_bounds__(kCombineThreads) serve_attention_combine_kernel(const ServeAttentionParams p, int ctas, int halves) {
@@ -1035,7 +1015,7 @@ __global__ void __launch_bounds__(kCombineThreads) serve_attention_combine_kerne
   const int cta = blockIdx.x;
   const Unfinished u = parts.unfinished[cta];
   if (u.valid == 0) return;
-  const int tokens_per_half = kRows / p.group;
+  const int tokens_per_half = p.tokens_per_tile;
   const int lane = threadIdx.x & 31;
   constexpr int kColumnGroups = kDim / 16;  // a warp takes 8 rows x 4 x 4 columns
   for (int unit = blockIdx.y * (kCombineThreads / 32) + threadIdx.x / 32; unit < halves * (kRows / 8) * kColumnGroups;

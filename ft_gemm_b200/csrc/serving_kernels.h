@@ -60,6 +60,7 @@ struct ServeAttentionParams {
   int mask_words, mask_stride;
   int batch, query_tokens, key_tokens;
   int heads, kv_heads, group, head_dim, causal;
+  int tokens_per_tile;  // 128 / group: tokens whose heads fill a tile of 128 rows
   int page_size, pages, table_pages, table_stride;
   int min_share;     // key tiles that a CTA takes at least
   float scale_log2;  // log2(e) * scale

@@ -6,6 +6,7 @@ packed prompts of different lengths and `TreeAttention` that of new or drafted t
 memory and streams only; the reference has no counterpart to any of them.
 """
 import ctypes
+import struct
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -44,7 +45,14 @@ class FtTreeAttentionArgs(ctypes.Structure):
         ("scale", ctypes.c_float)]
 
 
+# The same structures for the calls below, packed in one step: field by field they take longer than a small kernel runs.
+_ROWS = "Pqqi4x"
+_PACK_ROWS = struct.Struct(_ROWS).pack
+_PACK_PROMPT = struct.Struct(_ROWS * 4 + "PPPiiiiiif0P").pack
+_PACK_TREE = struct.Struct(_ROWS * 2 + "PPPPPiiiiiiif0P").pack
+
 _bound = False
+_calls = {}  # the entry points that run on a device, with structures given as packed bytes
 
 
 def _lib():
@@ -78,26 +86,26 @@ def _lib():
         lib.ft_prompt_attention_run.argtypes = [ctypes.POINTER(FtPromptAttentionArgs), vp, ctypes.c_size_t, vp, vp]
         lib.ft_tree_attention_run.argtypes = [cache, ctypes.POINTER(FtTreeAttentionArgs), vp, ctypes.c_size_t, vp, vp]
         lib.ft_tree_mask.argtypes = [ints, ci, ctypes.POINTER(ctypes.c_uint32), ci]
+        size = ctypes.c_size_t
+        for name, types in (("ft_rotary_run", [vp] * 6 + [ci] * 3 + [vp]), ("ft_kv_cache_append", [vp, ci, vp, vp, vp, ci] + [vp] * 5),
+                            ("ft_kv_cache_copy_pages", [vp, vp, vp, ci, vp]),
+                            ("ft_kv_cache_accept", [vp, vp, ci, ci, vp, vp, vp, vp, ci, vp, vp]),
+                            ("ft_prompt_attention_run", [vp, vp, size, vp, vp]), ("ft_tree_attention_run", [vp, vp, vp, size, vp, vp])):
+            _calls[name] = lib[name]
+            _calls[name].argtypes = types
         _bound = True
     return lib
 
 
-class _On:
-    """Makes a tensor's device current for a call, at no cost where it is already."""
-
-    def __init__(self, device: torch.device):
-        self.index = device.index
-        self.before = None
-
-    def __enter__(self):
-        now = torch.cuda.current_device()
-        if now != self.index:
-            self.before = now
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *error):
-        if self.before is not None:
-            torch.cuda.set_device(self.before)
+def _call(name: str, device: torch.device, *args):
+    """One of _calls on the device of its tensors, which is nearly always the current one already."""
+    if torch._C._cuda_getDevice() == device.index:
+        code = _calls[name](*args)
+    else:
+        with torch.cuda.device(device):
+            code = _calls[name](*args)
+    if code:
+        _abi.check(code)
 
 
 def _stream(device: torch.device, stream: Optional[torch.cuda.Stream]) -> int:
@@ -108,25 +116,28 @@ def _stream(device: torch.device, stream: Optional[torch.cuda.Stream]) -> int:
     return stream.cuda_stream
 
 
-def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, heads: int, head_dim: int, tokens: int) -> FtRows:
-    """[tokens, heads, head_dim] of the operator's type, head_dim contiguous; the C side checks alignment and strides."""
-    shape, stride = t.shape, t.stride()
-    if t.dtype != dtype or t.device != device or shape != (tokens, heads, head_dim) or stride[2] != 1:
+def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, heads: int, head_dim: int, tokens: int) -> Tuple[int, int, int, int]:
+    """The fields of an ft_rows: [tokens, heads, head_dim] of the operator's type, head_dim contiguous; the C side checks
+    alignment and strides."""
+    stride = t.stride()
+    if t.dtype is not dtype or t.get_device() != device.index or t.shape != (tokens, heads, head_dim) or stride[2] != 1:
         raise ValueError(f"{name} must be a [{tokens}, {heads}, {head_dim}] {dtype} tensor on {device} with a contiguous last dimension "
-                         f"(got {list(shape)}, {t.dtype} on {t.device}, strides {list(stride)})")
-    return FtRows(t.data_ptr(), stride[0], stride[1], heads)
+                         f"(got {list(t.shape)}, {t.dtype} on {t.device}, strides {list(stride)})")
+    return t.data_ptr(), stride[0], stride[1], heads
 
 
 def _vector(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, size: Optional[int] = None) -> int:
-    if t.dtype != dtype or t.device != device or t.dim() != 1 or not t.is_contiguous() or (size is not None and t.shape[0] != size):
+    if t.dtype is not dtype or t.get_device() != device.index or t.dim() != 1 or not t.is_contiguous() or (size is not None and len(t) != size):
         raise ValueError(f"{name} must be a contiguous one-dimensional {dtype} tensor on {device}" + (f" of {size} elements" if size is not None else ""))
     return t.data_ptr()
 
 
-def _matrix(t: torch.Tensor, name: str, device: torch.device, rows: int) -> int:
-    if t.dtype != torch.int32 or t.device != device or t.dim() != 2 or t.shape[0] != rows or t.shape[1] == 0 or t.stride(1) != 1:
+def _matrix(t: torch.Tensor, name: str, device: torch.device, rows: int) -> Tuple[int, int, int]:
+    """(address, columns, elements from row to row)"""
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not torch.int32 or t.get_device() != device.index or len(shape) != 2 or shape[0] != rows or shape[1] == 0 or stride[1] != 1:
         raise ValueError(f"{name} must be a [{rows}, columns] int32 tensor on {device} with contiguous rows")
-    return t.data_ptr()
+    return t.data_ptr(), shape[1], max(stride[0], shape[1]) if rows == 1 else stride[0]
 
 
 def _check_dtype(dtype: torch.dtype) -> int:
@@ -175,17 +186,20 @@ class Rotary:
             raise ValueError(f"q must be a [tokens, heads, {self.head_dim}] tensor on {self.device}")
         if (k is None) != (k_out is None):
             raise ValueError("k and k_out come together")
-        rq = _rows(q, "q", dtype, device, q.shape[1], self.head_dim, tokens)
-        ro = _rows(q_out, "q_out", dtype, device, q.shape[1], self.head_dim, tokens)
+        heads = q.shape[1]
+        rq = _PACK_ROWS(*_rows(q, "q", dtype, device, heads, self.head_dim, tokens))
+        ro = _PACK_ROWS(*_rows(q_out, "q_out", dtype, device, heads, self.head_dim, tokens))
         rk = rko = None
         if k is not None:
-            rk = _rows(k, "k", dtype, device, k.shape[1], self.head_dim, tokens)
-            rko = _rows(k_out, "k_out", dtype, device, k.shape[1], self.head_dim, tokens)
+            if k.dim() != 3:
+                raise ValueError(f"k must be a [{tokens}, heads, {self.head_dim}] tensor")
+            heads = k.shape[1]
+            rk = _PACK_ROWS(*_rows(k, "k", dtype, device, heads, self.head_dim, tokens))
+            rko = _PACK_ROWS(*_rows(k_out, "k_out", dtype, device, heads, self.head_dim, tokens))
         at = _vector(positions, "positions", torch.int64, device, tokens)
         if tokens == 0:
             return
-        with _On(device):
-            _abi.check(self.lib.ft_rotary_run(self.handle, rq, ro, rk, rko, at, tokens, code, int(inverse), _stream(device, stream)))
+        _call("ft_rotary_run", device, self.handle, rq, ro, rk, rko, at, tokens, code, int(inverse), _stream(device, stream))
 
     def close(self):
         if getattr(self, "handle", None) is not None and self.handle.value:
@@ -213,8 +227,8 @@ class PagedCache:
         self.layers, self.pages, self.page_size, self.kv_heads, self.head_dim = k.shape
         s = k.stride()
         self.view = FtKvCache(k.data_ptr(), v.data_ptr(), s[0], s[1], s[2], s[3], *k.shape, _check_dtype(k.dtype))
-        self._no_pairs = torch.empty(0, dtype=torch.int32, device=self.device)
-        self.copy_pages(self._no_pairs, self._no_pairs)  # refuses a layout that the kernels cannot take
+        _abi.check(self.lib.ft_kv_cache_copy_pages(ctypes.byref(self.view), None, None, 0, None))  # refuses a layout that the kernels cannot take
+        self.address = ctypes.addressof(self.view)
 
     @classmethod
     def empty(cls, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -227,32 +241,32 @@ class PagedCache:
         """Writes k and v [tokens, key heads, head_dim] to slots (int64: page * page_size + place; negative: not written;
         all different).  With `rotary`, K is rotated at `positions` on the way and q, if given, into q_out."""
         tokens = k.shape[0]
-        rk = _rows(k, "k", self.dtype, self.device, self.kv_heads, self.head_dim, tokens)
-        rv = _rows(v, "v", self.dtype, self.device, self.kv_heads, self.head_dim, tokens)
-        to = _vector(slots, "slots", torch.int64, self.device, tokens)
+        dtype, device, head_dim = self.dtype, self.device, self.head_dim
+        rk = _PACK_ROWS(*_rows(k, "k", dtype, device, self.kv_heads, head_dim, tokens))
+        rv = _PACK_ROWS(*_rows(v, "v", dtype, device, self.kv_heads, head_dim, tokens))
+        to = _vector(slots, "slots", torch.int64, device, tokens)
         handle = at = rq = ro = None
         if (q is None) != (q_out is None) or (rotary is None) != (positions is None) or (q is not None and rotary is None):
             raise ValueError("q and q_out come together, rotary and positions too, and q only with rotary")
         if rotary is not None:
-            if rotary.device != self.device or rotary.head_dim != self.head_dim:
-                raise ValueError(f"the rotary positions must be on {self.device} for heads of {self.head_dim}")
-            handle, at = rotary.handle, _vector(positions, "positions", torch.int64, self.device, tokens)
+            if rotary.device != device or rotary.head_dim != head_dim:
+                raise ValueError(f"the rotary positions must be on {device} for heads of {head_dim}")
+            handle, at = rotary.handle, _vector(positions, "positions", torch.int64, device, tokens)
         if q is not None:
             if q.dim() != 3:
                 raise ValueError("q must be [tokens, heads, head_dim]")
-            rq = _rows(q, "q", self.dtype, self.device, q.shape[1], self.head_dim, tokens)
-            ro = _rows(q_out, "q_out", self.dtype, self.device, q.shape[1], self.head_dim, tokens)
+            heads = q.shape[1]
+            rq = _PACK_ROWS(*_rows(q, "q", dtype, device, heads, head_dim, tokens))
+            ro = _PACK_ROWS(*_rows(q_out, "q_out", dtype, device, heads, head_dim, tokens))
         if tokens == 0:
             return
-        with _On(self.device):
-            _abi.check(self.lib.ft_kv_cache_append(self.view, layer, rk, rv, to, tokens, handle, at, rq, ro, _stream(self.device, stream)))
+        _call("ft_kv_cache_append", device, self.address, layer, rk, rv, to, tokens, handle, at, rq, ro, _stream(device, stream))
 
     def copy_pages(self, sources: torch.Tensor, targets: torch.Tensor, stream: Optional[torch.cuda.Stream] = None):
         """Copies page sources[i] to page targets[i] (int32) in every layer; no target may be a source or another target."""
         count = sources.shape[0]
         a, b = _vector(sources, "sources", torch.int32, self.device), _vector(targets, "targets", torch.int32, self.device, count)
-        with _On(self.device):
-            _abi.check(self.lib.ft_kv_cache_copy_pages(self.view, a, b, count, _stream(self.device, stream)))
+        _call("ft_kv_cache_copy_pages", self.device, self.address, a, b, count, _stream(self.device, stream))
 
     def accept(self, page_table: torch.Tensor, lengths: torch.Tensor, drafted_offsets: torch.Tensor, accepted: torch.Tensor,
                accepted_offsets: torch.Tensor, new_lengths: torch.Tensor, stream: Optional[torch.cuda.Stream] = None):
@@ -260,18 +274,17 @@ class PagedCache:
         accepted[accepted_offsets[b] + i] (ascending) to the i-th place behind the tokens that were there before them, in every
         layer, and writes the lengths that result.  All int32; page_table [batch, pages]."""
         batch = lengths.shape[0]
-        table = _matrix(page_table, "page_table", self.device, batch)
-        vectors = [_vector(lengths, "lengths", torch.int32, self.device), _vector(drafted_offsets, "drafted_offsets", torch.int32, self.device, batch + 1),
-                   _vector(accepted, "accepted", torch.int32, self.device),
-                   _vector(accepted_offsets, "accepted_offsets", torch.int32, self.device, batch + 1)]
+        table, columns, stride = _matrix(page_table, "page_table", self.device, batch)
+        held = _vector(lengths, "lengths", torch.int32, self.device)
+        offsets = _vector(drafted_offsets, "drafted_offsets", torch.int32, self.device, batch + 1)
+        nodes = _vector(accepted, "accepted", torch.int32, self.device)
+        ends = _vector(accepted_offsets, "accepted_offsets", torch.int32, self.device, batch + 1)
         out = _vector(new_lengths, "new_lengths", torch.int32, self.device, batch)
         if batch == 0:
             return
-        if accepted.shape[0] == 0:  # an empty tensor has no address
-            vectors[2] = out
-        with _On(self.device):
-            _abi.check(self.lib.ft_kv_cache_accept(self.view, table, page_table.shape[1], page_table.stride(0), *vectors, batch, out,
-                                                   _stream(self.device, stream)))
+        # an empty tensor has no address, but then nothing is read there
+        _call("ft_kv_cache_accept", self.device, self.address, table, columns, stride, held, offsets, nodes or out, ends, batch, out,
+              _stream(self.device, stream))
 
 
 class PagePool:
@@ -320,7 +333,7 @@ class PagePool:
 
     def _move(self, pairs: List[Tuple[int, int]], stream: Optional[torch.cuda.Stream]):
         if pairs and self.cache is not None:
-            with torch.cuda.stream(stream) if stream is not None else _On(self.cache.device):
+            with torch.cuda.stream(stream) if stream is not None else torch.cuda.device(self.cache.device):
                 both = torch.tensor(pairs, dtype=torch.int32).t().contiguous().to(self.cache.device)
                 self.cache.copy_pages(both[0], both[1])
 
@@ -382,6 +395,7 @@ class _Attention:
         self.lib = _lib()
         self.device = torch.empty(0, device=device).device
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self.status_at = self.status.data_ptr()
         with torch.cuda.device(self.device):
             self.workspace_bytes = self.lib.ft_attention_workspace()
             # the status word is zero before any other stream can run a kernel that writes to it
@@ -390,9 +404,9 @@ class _Attention:
     def _workspace(self, stream: Optional[torch.cuda.Stream]) -> torch.Tensor:
         """A workspace of this call's own, from the caller's allocator, on the stream that uses it."""
         if stream is None:
-            return torch.empty(self.workspace_bytes, dtype=torch.uint8, device=self.device)
+            return self.status.new_empty(self.workspace_bytes // 4)
         with torch.cuda.stream(stream):
-            return torch.empty(self.workspace_bytes, dtype=torch.uint8, device=self.device)
+            return self.status.new_empty(self.workspace_bytes // 4)
 
     def report(self):
         """Waits for the device and raises if a device-side wait of an earlier run gave up: its output is not valid."""
@@ -409,8 +423,7 @@ class PromptAttention(_Attention):
 
     def __init__(self, heads: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16, causal: bool = True, scale: float = 0.0,
                  device="cuda"):
-        a = self.args = FtPromptAttentionArgs()
-        a.dtype, a.head_dim, a.causal, a.scale = _check_dtype(dtype), head_dim, int(causal), scale
+        self.code, self.causal, self.scale = _check_dtype(dtype), int(causal), scale
         self.heads, self.kv_heads, self.head_dim, self.dtype = heads, kv_heads, head_dim, dtype
         self._begin(device)
 
@@ -418,24 +431,20 @@ class PromptAttention(_Attention):
             key_offsets: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None):
         """offsets, key_offsets (None: the same): int32 [sequences + 1]; lse: float32 [tokens, heads] or None.  Rows of out
         behind the last sequence are left as they are."""
-        device, tokens, keys = self.device, q.shape[0], k.shape[0]
-        a = FtPromptAttentionArgs.from_buffer_copy(self.args)  # each call its own: host threads may share the operator
-        a.q = _rows(q, "q", self.dtype, device, self.heads, self.head_dim, tokens)
-        a.k = _rows(k, "k", self.dtype, device, self.kv_heads, self.head_dim, keys)
-        a.v = _rows(v, "v", self.dtype, device, self.kv_heads, self.head_dim, keys)
-        a.out = _rows(out, "out", self.dtype, device, self.heads, self.head_dim, tokens)
-        a.batch = offsets.shape[0] - 1
-        a.q_offsets = _vector(offsets, "offsets", torch.int32, device)
+        dtype, device, heads, kv_heads, head_dim, tokens, keys = self.dtype, self.device, self.heads, self.kv_heads, self.head_dim, len(q), len(k)
+        rows = _rows(q, "q", dtype, device, heads, head_dim, tokens) + _rows(k, "k", dtype, device, kv_heads, head_dim, keys) + _rows(
+            v, "v", dtype, device, kv_heads, head_dim, keys) + _rows(out, "out", dtype, device, heads, head_dim, tokens)
+        batch = len(offsets) - 1
+        at = _vector(offsets, "offsets", torch.int32, device)
         if key_offsets is None and keys != tokens:
             raise ValueError("key_offsets are needed where q and k differ in tokens")
-        a.k_offsets = None if key_offsets is None else _vector(key_offsets, "key_offsets", torch.int32, device, a.batch + 1)
-        a.query_tokens, a.key_tokens = tokens, keys
-        a.lse = _lse(lse, device, tokens, self.heads)
-        if a.batch <= 0 or tokens == 0:
+        key_at = 0 if key_offsets is None else _vector(key_offsets, "key_offsets", torch.int32, device, batch + 1)
+        lse_at = 0 if lse is None else _lse(lse, device, tokens, heads)
+        if batch <= 0 or tokens == 0:
             return
-        with _On(device):
-            workspace = self._workspace(stream)
-            _abi.check(self.lib.ft_prompt_attention_run(a, workspace.data_ptr(), self.workspace_bytes, self.status.data_ptr(), _stream(device, stream)))
+        args = _PACK_PROMPT(*rows, lse_at, at, key_at, batch, tokens, keys, head_dim, self.code, self.causal, self.scale)
+        workspace = self._workspace(stream)
+        _call("ft_prompt_attention_run", device, args, workspace.data_ptr(), self.workspace_bytes, self.status_at, _stream(device, stream))
 
 
 class TreeAttention(_Attention):
@@ -444,8 +453,7 @@ class TreeAttention(_Attention):
 
     def __init__(self, heads: int, cache: PagedCache, scale: float = 0.0):
         self.cache, self.heads = cache, heads
-        self.args = FtTreeAttentionArgs()
-        self.args.scale = scale
+        self.scale = scale
         self._begin(cache.device)
 
     def run(self, q: torch.Tensor, layer: int, offsets: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, out: torch.Tensor,
@@ -453,33 +461,22 @@ class TreeAttention(_Attention):
         """Sequence b holds lengths[b] tokens in the pages of page_table[b]; the queries of its last offsets[b+1] - offsets[b]
         ones are q[offsets[b]:offsets[b+1]].  They see every token before them, and of themselves what the mask says: int32 words
         [tokens, words], bit j of a row is set where the row sees new token j of its sequence; None: each sees up to itself."""
-        cache, device, tokens = self.cache, self.device, q.shape[0]
-        a = FtTreeAttentionArgs.from_buffer_copy(self.args)  # each call its own: host threads may share the operator
-        a.q = _rows(q, "q", cache.dtype, device, self.heads, cache.head_dim, tokens)
-        a.out = _rows(out, "out", cache.dtype, device, self.heads, cache.head_dim, tokens)
-        a.batch = offsets.shape[0] - 1
-        a.q_offsets = _vector(offsets, "offsets", torch.int32, device)
-        a.page_table = _matrix(page_table, "page_table", device, a.batch)
-        a.table_pages, a.table_stride = page_table.shape[1], max(page_table.stride(0), page_table.shape[1])
-        a.lengths = _vector(lengths, "lengths", torch.int32, device, a.batch)
-        if mask is None:
-            a.mask = None
-        else:
-            a.mask = _matrix(mask, "mask", device, tokens)
-            a.mask_words, a.mask_stride = mask.shape[1], max(mask.stride(0), mask.shape[1])
-        a.query_tokens, a.layer = tokens, layer
-        a.lse = _lse(lse, device, tokens, self.heads)
-        if a.batch <= 0 or tokens == 0:
+        cache, device, heads, tokens = self.cache, self.device, self.heads, len(q)
+        rows = _rows(q, "q", cache.dtype, device, heads, cache.head_dim, tokens) + _rows(out, "out", cache.dtype, device, heads, cache.head_dim, tokens)
+        batch = len(offsets) - 1
+        at = _vector(offsets, "offsets", torch.int32, device)
+        table, columns, table_stride = _matrix(page_table, "page_table", device, batch)
+        held = _vector(lengths, "lengths", torch.int32, device, batch)
+        mask_at, words, mask_stride = (0, 0, 0) if mask is None else _matrix(mask, "mask", device, tokens)
+        lse_at = 0 if lse is None else _lse(lse, device, tokens, heads)
+        if batch <= 0 or tokens == 0:
             return
-        with _On(device):
-            workspace = self._workspace(stream)
-            _abi.check(self.lib.ft_tree_attention_run(cache.view, a, workspace.data_ptr(), self.workspace_bytes, self.status.data_ptr(),
-                                                      _stream(device, stream)))
+        args = _PACK_TREE(*rows, lse_at, at, table, held, mask_at, words, mask_stride, batch, tokens, columns, table_stride, layer, self.scale)
+        workspace = self._workspace(stream)
+        _call("ft_tree_attention_run", device, cache.address, args, workspace.data_ptr(), self.workspace_bytes, self.status_at, _stream(device, stream))
 
 
-def _lse(lse: Optional[torch.Tensor], device: torch.device, tokens: int, heads: int) -> Optional[int]:
-    if lse is None:
-        return None
+def _lse(lse: torch.Tensor, device: torch.device, tokens: int, heads: int) -> int:
     if lse.dtype != torch.float32 or lse.device != device or lse.shape != (tokens, heads) or not lse.is_contiguous():
         raise ValueError(f"lse must be a contiguous float32 [{tokens}, {heads}] tensor on {device}")
     return lse.data_ptr()
