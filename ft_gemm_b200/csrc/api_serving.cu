@@ -592,7 +592,7 @@ static int check_workspace(const void* workspace, size_t bytes, const int* statu
 
 // What both calls share: the rows of q and out, the launch.
 static int attention_run(ServeAttentionParams& p, const ft_rows& q, const ft_rows& out, const CUtensorMap& k_map, const CUtensorMap& v_map, int dtype,
-                         float scale, void* workspace, size_t workspace_bytes, int* status, int sm_count, void* stream) {
+                         long long most_keys, float scale, void* workspace, size_t workspace_bytes, int* status, int sm_count, void* stream) {
   if (workspace_bytes < serve_attention_workspace(sm_count)) {
     return noalloc_fail(FT_ERR_INVALID, "the workspace holds %zu bytes, ft_attention_workspace() says %zu", workspace_bytes,
                         serve_attention_workspace(sm_count));
@@ -610,10 +610,14 @@ static int attention_run(ServeAttentionParams& p, const ft_rows& q, const ft_row
   p.min_share = 1;
   p.workspace = workspace;
   p.status = status;
-  // Two row tiles per CTA halve the reads of K and V, which pays once there are enough row tiles for every SM.
-  const long long pairs = (static_cast<long long>(p.query_tokens) * p.group + 255) / 256 * p.kv_heads;
-  const bool split_keys = pairs < sm_count;
-  SERVE_CUDA(launch_serve_attention(q_map, k_map, v_map, p, dtype, split_keys, sm_count, static_cast<cudaStream_t>(stream)));
+  // Two tiles of rows that go through the keys together halve what is read of K and V.  That needs sequences of more than
+  // one tile, and enough key tiles for every SM; below that the finer items fill the SMs better.  (Only sizes that the
+  // host knows go into this: averages over the sequences, and the most keys there can be.)  B200, 32 heads of 128 on 8: trees of 64 and
+  // 31 tokens over 131072 and 65001 keys 223 us split, 194 us in pairs; a prompt of 200 tokens 11.3 and 16.4 us; 64 single tokens
+  // over up to 8060 keys 69 and 89 us.
+  const long long tiles = (static_cast<long long>(p.query_tokens) + p.tokens_per_tile - 1) / p.tokens_per_tile;
+  const bool pairs = tiles > p.batch && tiles * p.kv_heads * (most_keys / 128 + 1) >= 4ll * sm_count;
+  SERVE_CUDA(launch_serve_attention(q_map, k_map, v_map, p, dtype, !pairs, sm_count, static_cast<cudaStream_t>(stream)));
   return FT_OK;
 }
 
@@ -663,7 +667,7 @@ int ft_prompt_attention_run(const ft_prompt_attention_args* a, void* workspace, 
   p.kv_heads = a->k.heads;
   p.head_dim = a->head_dim;
   p.causal = a->causal != 0;
-  return attention_run(p, a->q, a->out, maps[0], maps[1], a->dtype, a->scale, workspace, workspace_bytes, status, sm_count, stream);
+  return attention_run(p, a->q, a->out, maps[0], maps[1], a->dtype, a->key_tokens / a->batch, a->scale, workspace, workspace_bytes, status, sm_count, stream);
 }
 
 int ft_tree_attention_run(const ft_kv_cache* cache, const ft_tree_attention_args* a, void* workspace, size_t workspace_bytes, int* status,
@@ -720,7 +724,7 @@ int ft_tree_attention_run(const ft_kv_cache* cache, const ft_tree_attention_args
   p.pages = cache->pages;
   p.table_pages = a->table_pages;
   p.table_stride = a->table_stride;
-  return attention_run(p, a->q, a->out, maps[0], maps[1], cache->dtype, a->scale, workspace, workspace_bytes, status, sm_count, stream);
+  return attention_run(p, a->q, a->out, maps[0], maps[1], cache->dtype, static_cast<long long>(a->table_pages) * cache->page_size, a->scale, workspace, workspace_bytes, status, sm_count, stream);
 }
 
 int ft_tree_mask(const int* parents, int nodes, uint32_t* mask, int words) {
