@@ -326,7 +326,7 @@ int ft_kv_cache_append(const ft_kv_cache* cache, int layer, const ft_rows* k, co
   p.page_stride = cache->page_stride;
   p.cache_token_stride = cache->token_stride;
   p.cache_head_stride = cache->head_stride;
-  p.page_size = cache->page_size;
+  while ((1 << p.page_shift) < cache->page_size) ++p.page_shift;
   p.slot_count = static_cast<long long>(cache->pages) * cache->page_size;
   p.tokens = tokens;
   SERVE_CUDA(launch_rotary(p, cache->dtype, static_cast<cudaStream_t>(stream)));

@@ -74,6 +74,9 @@ struct Layout {
   static constexpr int kSlabs = kDim / 64;              // 128-byte columns of a row of Q, K or V
   static constexpr int kTileBytes = kSlabs * 128 * 128;
   static constexpr int kQTiles = kSplitKeys ? 1 : 2;
+  // What a row tile costs beside its key tiles, in key tiles (us at 1, 2, 3 and 4): 64 single tokens over up to 8060 keys 82, 70, 75, 79;
+  // ragged prompts in pairs 53.8, 55.4, 57.7, 60.2.
+  static constexpr int kItemCost = kSplitKeys ? 2 : 1;
   static constexpr int kStages = kDim == 64 ? 10 : kSplitKeys ? 5 : 4;
   static constexpr int kBytes = (kQTiles + kStages) * kTileBytes + static_cast<int>(sizeof(Shared)) + 1024;
   static_assert(kBytes <= 232448 && kStages <= kMaxStages, "shared memory of one CTA");
@@ -212,7 +215,7 @@ __device__ __forceinline__ RawSequence load_raw(const ServeAttentionParams& p, i
   r.k_end = p.page_table != nullptr ? p.lengths[b] : p.k_offsets[b + 1];
   return r;
 }
-__device__ __forceinline__ Sequence make_sequence(const ServeAttentionParams& p, const RawSequence& r, int tokens_per_item) {
+__device__ __forceinline__ Sequence make_sequence(const ServeAttentionParams& p, const RawSequence& r, int tokens_per_item, int item_cost) {
   Sequence s;
   s.token0 = min(max(r.q_begin, 0), p.query_tokens);
   const int queries = min(max(r.q_end, s.token0), p.query_tokens) - s.token0;
@@ -225,12 +228,12 @@ __device__ __forceinline__ Sequence make_sequence(const ServeAttentionParams& p,
     s.key_row0 = min(max(r.k_begin, 0), p.key_tokens);
     keys = full = min(max(r.k_end, s.key_row0), p.key_tokens) - s.key_row0;
   }
-  s.tiles = SequenceTiles::make(queries, keys, full, tokens_per_item, p.causal != 0 && p.mask == nullptr);
+  s.tiles = SequenceTiles::make(queries, keys, full, tokens_per_item, item_cost, p.causal != 0 && p.mask == nullptr);
   return s;
 }
 
-__device__ __forceinline__ Sequence load_sequence(const ServeAttentionParams& p, int b, int tokens_per_item) {
-  return make_sequence(p, load_raw(p, b), tokens_per_item);
+__device__ __forceinline__ Sequence load_sequence(const ServeAttentionParams& p, int b, int tokens_per_item, int item_cost) {
+  return make_sequence(p, load_raw(p, b), tokens_per_item, item_cost);
 }
 
 __device__ __forceinline__ Item load_item(const volatile Item& from) {
@@ -339,7 +342,7 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll 1
       for (int i = scan_begin; i < scan_end; ++i) {
-        seq = load_sequence(p, i, tokens_per_item);
+        seq = load_sequence(p, i, tokens_per_item, L::kItemCost);
         per_head = seq.tiles.units_per_head();
         const long long units = per_head * p.kv_heads;
         if (pass == 0) {
@@ -379,6 +382,7 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       seq.tiles.prefix = __shfl_sync(0xffffffffU, seq.tiles.prefix, owner);
       seq.tiles.row_tiles = __shfl_sync(0xffffffffU, seq.tiles.row_tiles, owner);
       seq.tiles.tokens_per_item = tokens_per_item;
+      seq.tiles.item_cost = L::kItemCost;
       seq.tiles.chain = chain;
       seq.tiles.ramp = __shfl_sync(0xffffffffU, seq.tiles.ramp ? 1 : 0, owner) != 0;
     }
@@ -418,7 +422,7 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         }
         row_tile = lo;
         first = static_cast<int>(inner - in_front);
-        if (first <= kItemCost) {  // the whole row tile is this CTA's, whatever lies in front of the boundary
+        if (first <= L::kItemCost) {  // the whole row tile is this CTA's, whatever lies in front of the boundary
           left += first;
           first = 0;
         }
@@ -430,7 +434,7 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         if (!ok) break;
         Item item = {};
         const int units = left > 0 ? seq.tiles.units_of(row_tile) : 0;
-        if (left <= 0 || (first == 0 && left <= kItemCost && left < units)) {  // the next CTA takes a row tile that would only begin here
+        if (left <= 0 || (first == 0 && left <= L::kItemCost && left < units)) {  // the next CTA takes a row tile that would only begin here
           item.tokens = -1;
           if (lane == 0) {
             sh.items[slot_index] = item;
@@ -447,8 +451,8 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         item.keys = seq.tiles.keys;
         item.limit = seq.tiles.limit(item.place0 + item.tokens);
         const int real = item.limit <= 0 ? 0 : (item.limit - 1) / kKeyTile + 1;  // a unit may have no key tile in it
-        item.first = min(max(first - kItemCost, 0), real);
-        item.end = min(max(end - kItemCost, 0), real);
+        item.first = min(max(first - L::kItemCost, 0), real);
+        item.end = min(max(end - L::kItemCost, 0), real);
         item.slot = first == 0 && end == units ? -1 : first > 0 ? 0 : 1;
         if (first == 0 && end < units) {
           unfinished.valid = 1;
@@ -543,7 +547,7 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             kv_head = 0;
             do {
               ++b;
-              seq = make_sequence(p, next, tokens_per_item);
+              seq = make_sequence(p, next, tokens_per_item, L::kItemCost);
               next = load_raw(p, min(b + 1, p.batch - 1));
             } while (seq.tiles.row_tiles == 0 && b + 1 < p.batch);
           }

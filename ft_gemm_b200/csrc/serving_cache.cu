@@ -22,20 +22,101 @@ union Chunk {  // 16 bytes: eight elements
   T pairs[4];
 };
 
-constexpr int kRotaryThreads = 256;
 
-// Rotates, copies and scatters the rows of `tokens_per_block` tokens.  A thread takes two 16-byte chunks of one row: the
+// Rotates, copies and scatters the rows of `tokens_per_block` tokens.  A thread takes two 16-byte chunks of a row: the
 // two halves of eight pairs (or, interleaved, eight pairs outright), or two chunks that are only copied.  Sines and cosines
-// are computed once per token and frequency, shared by all heads: the angle in turns is position * frequency / 2pi, formed
-// and reduced to [-1/2, 1/2] in 64 bits (32 bits lose it beyond some ten thousand positions), then one sincospi in 32 bits.
-template <typename T>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryParams p, int tokens_per_block) {
+// are computed once per token and frequency, shared by all heads, while the first rows are on their way: the angle in
+// turns is position * frequency / 2pi, formed and reduced to [-1/2, 1/2] in 64 bits (32 bits lose it beyond some ten
+// thousand positions), then one sincospi in 32 bits.
+// Bound by HBM for many tokens: 16384 tokens of 32 + 8 heads of 128 with the append, 403 MB, in 64 us = 6.3 TB/s (0.96 of the
+// measured copy rate); of the shapes tried (128 to 512 threads, 1 to 8 tokens a block, 1 to 3 rows in flight per thread: 64
+// to 100 us) many resident warps with one row each are the fastest.
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p, int tokens_per_block) {
   extern __shared__ float2 turn[];  // [token in block][rotary_dim / 2]: magnitude * (cos, sin)
   const int half = p.rotary_dim / 2;
   const int first = blockIdx.x * tokens_per_block;
   const int count = min(tokens_per_block, p.tokens - first);
-  const int thread = threadIdx.y * blockDim.x + threadIdx.x;
-  for (int i = thread; i < count * half; i += blockDim.x * blockDim.y) {
+  const int rows = p.q_heads + p.k_heads + p.v_heads;
+  const int unit = threadIdx.x;  // which two chunks of the row
+  const int rotated_units = p.rotary_dim / 16;
+
+  struct Work {
+    uint16_t* dst;  // nullptr: nothing to do
+    int token;      // in the block
+    bool rotate;
+    Chunk<T> a, b;
+  };
+  auto places = [&](bool rotate, int& at0, int& at1) {
+    const bool halves = rotate && !p.interleaved;
+    at0 = halves ? unit * 8 : unit * 16;
+    at1 = halves ? at0 + half : at0 + 8;
+  };
+  auto load = [&](int r, Work& w) {
+    w.dst = nullptr;
+    if (r >= count * rows) return;
+    w.token = r / rows;
+    int head = r - w.token * rows;
+    const long long token = first + w.token;
+    const uint16_t* src;
+    w.rotate = unit < rotated_units;
+    if (head < p.q_heads) {
+      src = p.q.data + token * p.q.token_stride + head * p.q.head_stride;
+      w.dst = p.q_out.data + token * p.q_out.token_stride + head * p.q_out.head_stride;
+    } else {
+      head -= p.q_heads;
+      const bool value = head >= p.k_heads;
+      if (value) {
+        head -= p.k_heads;
+        w.rotate = false;
+      }
+      const Rows& rows_in = value ? p.v : p.k;
+      src = rows_in.data + token * rows_in.token_stride + head * rows_in.head_stride;
+      if (p.slots != nullptr) {
+        const long long slot = p.slots[token];
+        if (slot < 0 || slot >= p.slot_count) return;  // padding of the batch
+        w.dst = (value ? p.v_cache : p.k_cache) + (slot >> p.page_shift) * p.page_stride + (slot & ((1 << p.page_shift) - 1)) * p.cache_token_stride +
+                head * p.cache_head_stride;
+      } else {
+        w.dst = p.k_out.data + token * p.k_out.token_stride + head * p.k_out.head_stride;
+      }
+    }
+    int at0, at1;
+    places(w.rotate, at0, at1);
+    w.a.raw = *reinterpret_cast<const uint4*>(src + at0);
+    w.b.raw = *reinterpret_cast<const uint4*>(src + at1);
+  };
+  auto finish = [&](Work& w) {
+    if (w.dst == nullptr) return;
+    if (w.rotate) {
+      const float2* cs = turn + w.token * half + unit * 8;
+      if (p.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 x = unpack(w.a.pairs[i]), y = unpack(w.b.pairs[i]);
+          const float2 u = cs[i], v = cs[4 + i];
+          pack(w.a.pairs[i], x.x * u.x - x.y * u.y, x.x * u.y + x.y * u.x);
+          pack(w.b.pairs[i], y.x * v.x - y.y * v.y, y.x * v.y + y.y * v.x);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 x = unpack(w.a.pairs[i]), y = unpack(w.b.pairs[i]);
+          const float2 u = cs[2 * i], v = cs[2 * i + 1];
+          pack(w.a.pairs[i], x.x * u.x - y.x * u.y, x.y * v.x - y.y * v.y);
+          pack(w.b.pairs[i], x.x * u.y + y.x * u.x, x.y * v.y + y.y * v.x);
+        }
+      }
+    }
+    int at0, at1;
+    places(w.rotate, at0, at1);
+    *reinterpret_cast<uint4*>(w.dst + at0) = w.a.raw;
+    *reinterpret_cast<uint4*>(w.dst + at1) = w.b.raw;
+  };
+
+  Work work;
+  load(threadIdx.y, work);
+  for (int i = threadIdx.y * blockDim.x + threadIdx.x; i < count * half; i += blockDim.x * blockDim.y) {
     const int t = i / half, f = i - t * half;
     double angle = static_cast<double>(p.positions[first + t]) * p.turns[f];
     angle -= rint(angle);
@@ -44,65 +125,10 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
     turn[i] = make_float2(c * p.magnitude, (p.inverse ? -s : s) * p.magnitude);
   }
   __syncthreads();
-
-  const int rows = p.q_heads + p.k_heads + p.v_heads;
-  const int unit = threadIdx.x;  // which two chunks of the row
-  const int rotated_units = p.rotary_dim / 16;
-  for (int r = threadIdx.y; r < count * rows; r += blockDim.y) {
-    const int t = r / rows;
-    int head = r - t * rows;
-    const long long token = first + t;
-    const uint16_t* src;
-    uint16_t* dst;
-    bool rotate = unit < rotated_units;
-    if (head < p.q_heads) {
-      src = p.q.data + token * p.q.token_stride + head * p.q.head_stride;
-      dst = p.q_out.data + token * p.q_out.token_stride + head * p.q_out.head_stride;
-    } else {
-      head -= p.q_heads;
-      const bool value = head >= p.k_heads;
-      if (value) {
-        head -= p.k_heads;
-        rotate = false;
-      }
-      const Rows& rows_in = value ? p.v : p.k;
-      src = rows_in.data + token * rows_in.token_stride + head * rows_in.head_stride;
-      if (p.slots != nullptr) {
-        const long long slot = p.slots[token];
-        if (slot < 0 || slot >= p.slot_count) continue;  // padding of the batch
-        dst = (value ? p.v_cache : p.k_cache) + (slot / p.page_size) * p.page_stride + (slot % p.page_size) * p.cache_token_stride +
-              head * p.cache_head_stride;
-      } else {
-        dst = p.k_out.data + token * p.k_out.token_stride + head * p.k_out.head_stride;
-      }
-    }
-    const bool halves = rotate && !p.interleaved;
-    const int at0 = halves ? unit * 8 : unit * 16, at1 = halves ? at0 + half : at0 + 8;
-    Chunk<T> a, b;
-    a.raw = *reinterpret_cast<const uint4*>(src + at0);
-    b.raw = *reinterpret_cast<const uint4*>(src + at1);
-    if (rotate) {
-      const float2* cs = turn + t * half + unit * 8;
-      if (p.interleaved) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 x = unpack(a.pairs[i]), y = unpack(b.pairs[i]);
-          const float2 u = cs[i], w = cs[4 + i];
-          pack(a.pairs[i], x.x * u.x - x.y * u.y, x.x * u.y + x.y * u.x);
-          pack(b.pairs[i], y.x * w.x - y.y * w.y, y.x * w.y + y.y * w.x);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 x = unpack(a.pairs[i]), y = unpack(b.pairs[i]);
-          const float2 u = cs[2 * i], w = cs[2 * i + 1];
-          pack(a.pairs[i], x.x * u.x - y.x * u.y, x.y * w.x - y.y * w.y);
-          pack(b.pairs[i], x.x * u.y + y.x * u.x, x.y * w.y + y.y * w.x);
-        }
-      }
-    }
-    *reinterpret_cast<uint4*>(dst + at0) = a.raw;
-    *reinterpret_cast<uint4*>(dst + at1) = b.raw;
+  for (int r = threadIdx.y; r < count * rows;) {
+    finish(work);
+    r += blockDim.y;
+    load(r, work);
   }
 }
 
@@ -180,19 +206,26 @@ __global__ void __launch_bounds__(256) accept_kernel(const AcceptParams p) {
 
 }  // namespace
 
-cudaError_t launch_rotary(const RotaryParams& p, int dtype, cudaStream_t stream) {
+template <int kThreads>
+static cudaError_t launch_rotary_threads(const RotaryParams& p, int dtype, int tokens, cudaStream_t stream) {
   const int rows = p.q_heads + p.k_heads + p.v_heads;
-  if (p.tokens <= 0 || rows <= 0) return cudaSuccess;
-  const dim3 block(p.head_dim / 16, kRotaryThreads / (p.head_dim / 16));
-  const int tokens_per_block = std::min(16, std::max(1, static_cast<int>(block.y) / rows));
+  const dim3 block(p.head_dim / 16, kThreads / (p.head_dim / 16));
+  const int tokens_per_block = std::min(16, std::max(tokens, static_cast<int>(block.y) / rows));
   const int grid = (p.tokens + tokens_per_block - 1) / tokens_per_block;
   const size_t smem = static_cast<size_t>(tokens_per_block) * (p.rotary_dim / 2) * sizeof(float2);
   if (dtype == FT_SRC_BF16) {
-    rotary_kernel<__nv_bfloat162><<<grid, block, smem, stream>>>(p, tokens_per_block);
+    rotary_kernel<__nv_bfloat162, kThreads><<<grid, block, smem, stream>>>(p, tokens_per_block);
   } else {
-    rotary_kernel<__half2><<<grid, block, smem, stream>>>(p, tokens_per_block);
+    rotary_kernel<__half2, kThreads><<<grid, block, smem, stream>>>(p, tokens_per_block);
   }
   return cudaGetLastError();
+}
+
+cudaError_t launch_rotary(const RotaryParams& p, int dtype, cudaStream_t stream) {
+  if (p.tokens <= 0 || p.q_heads + p.k_heads + p.v_heads <= 0) return cudaSuccess;
+  // Few tokens: a block of many threads per token, so that its rows go in one or two rounds (64 tokens: 2.4 us with 512 threads, 3.0
+  // with 256).  Many: smaller blocks, of two tokens once that fills the SMs (16384 tokens: 64 us, 72 with 512 threads).
+  return p.tokens <= 512 ? launch_rotary_threads<512>(p, dtype, 1, stream) : launch_rotary_threads<256>(p, dtype, p.tokens >= 4096 ? 2 : 1, stream);
 }
 
 cudaError_t launch_copy_pages(const CopyPagesParams& p, cudaStream_t stream) {

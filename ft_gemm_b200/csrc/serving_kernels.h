@@ -22,7 +22,7 @@ struct RotaryParams {
   uint16_t *k_cache, *v_cache;
   long long page_stride, cache_token_stride, cache_head_stride;
   long long slot_count;
-  int page_size;
+  int page_shift;  // page_size = 1 << page_shift
   int tokens, head_dim, rotary_dim;
   int interleaved, inverse;
   float magnitude;

@@ -2,8 +2,8 @@
 // on the device and on the host (where it is tested).
 //
 // A sequence of n queries and some keys makes, for each key head, ceil(n / tokens_per_item) row tiles; a row tile works
-// through the 128-key tiles that any of its rows may see.  To begin and end a row tile costs about as much as kItemCost
-// key tiles, so a row tile of T key tiles is T + kItemCost units of work, the first kItemCost of them without a key tile.
+// through the 128-key tiles that any of its rows may see.  To begin and end a row tile costs about as much as item_cost
+// key tiles, so a row tile of T key tiles is T + item_cost units of work, the first item_cost of them without a key tile.
 // The units of all row tiles, heads and sequences are numbered in a row, and CTA c takes [c * share, (c + 1) * share); a
 // row tile whose first key tile lies in a share's front belongs to that share from its beginning.
 #pragma once
@@ -20,7 +20,6 @@
 namespace ftg {
 
 constexpr int kKeyTile = 128;
-constexpr int kItemCost = 2;
 
 FT_HD_CALL long long wide_quotient(long long a, long long b) { return a / b; }
 // 64-bit numbers that nearly always fit into 32 bits, where a division is several times cheaper
@@ -52,15 +51,17 @@ struct SequenceTiles {
   int prefix;           // key tokens in front of the first query's own (negative: the first queries see nothing)
   int row_tiles;        // per key head
   int tokens_per_item;
+  int item_cost;
   bool chain;           // query t sees keys [0, prefix + t]; otherwise row tiles count all keys
   bool ramp;            // row tiles are numbered with their own key limit; otherwise with all keys
 
-  FT_HD static SequenceTiles make(int queries, int keys, int full_keys, int tokens_per_item, bool chain) {
+  FT_HD static SequenceTiles make(int queries, int keys, int full_keys, int tokens_per_item, int item_cost, bool chain) {
     SequenceTiles s;
     s.queries = queries;
     s.keys = keys;
     s.prefix = full_keys - queries;
     s.tokens_per_item = tokens_per_item;
+    s.item_cost = item_cost;
     s.row_tiles = queries <= 0 ? 0 : (queries - 1) / tokens_per_item + 1;
     s.chain = chain;
     s.ramp = chain && keys == full_keys;
@@ -75,20 +76,20 @@ struct SequenceTiles {
   FT_HD static int tiles(int limit) { return limit <= 0 ? 1 : (limit - 1) / kKeyTile + 1; }
   // units of row tile r: at least one key tile, so that rows without keys are written too
   FT_HD int units_of(int r) const {
-    if (!ramp) return tiles(keys) + kItemCost;
+    if (!ramp) return tiles(keys) + item_cost;
     const long long end = static_cast<long long>(r + 1) * tokens_per_item;
-    return tiles(limit(end < queries ? static_cast<int>(end) : queries)) + kItemCost;
+    return tiles(limit(end < queries ? static_cast<int>(end) : queries)) + item_cost;
   }
   // units of the row tiles in front of r, r in [0, row_tiles]
   FT_HD long long units_before(int r) const {
-    if (!ramp) return static_cast<long long>(r) * (tiles(keys) + kItemCost);
+    if (!ramp) return static_cast<long long>(r) * (tiles(keys) + item_cost);
     const int inner = r < row_tiles ? r : row_tiles - 1;  // the last row tile ends with the queries, not on the line
     int empty = 0;                                        // row tiles that see nothing
     if (prefix < 0) {
       empty = -prefix / tokens_per_item;
       empty = empty > inner ? inner : empty;
     }
-    long long total = static_cast<long long>(inner) * kItemCost + empty + floor_sum(inner - empty, tokens_per_item, tokens_per_item * (empty + 1) + prefix + kKeyTile - 1);
+    long long total = static_cast<long long>(inner) * item_cost + empty + floor_sum(inner - empty, tokens_per_item, tokens_per_item * (empty + 1) + prefix + kKeyTile - 1);
     if (r == row_tiles && row_tiles > 0) total += units_of(row_tiles - 1);
     return total;
   }
