@@ -608,6 +608,11 @@ static int attention_run(ServeAttentionParams& p, const ft_rows& q, const ft_row
   p.tokens_per_tile = 128 / p.group;
   p.scale_log2 = 1.44269504088896340736f * (scale != 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(p.head_dim)));
   p.min_share = 1;
+  // an upper bound on the units of work (serving_schedule.h), which are numbered in 31 bits
+  const long long row_tiles = static_cast<long long>(p.query_tokens) / p.tokens_per_tile + p.batch;
+  if (row_tiles > INT32_MAX / 8 || row_tiles * p.kv_heads > INT32_MAX / (most_keys / 128 + 8)) {
+    return noalloc_fail(FT_ERR_INVALID, "the call is too large: %lld tiles of query rows for %d key heads over up to %lld keys", row_tiles, p.kv_heads, most_keys);
+  }
   p.workspace = workspace;
   p.status = status;
   // Two tiles of rows that go through the keys together halve what is read of K and V.  That needs sequences of more than
@@ -616,7 +621,8 @@ static int attention_run(ServeAttentionParams& p, const ft_rows& q, const ft_row
   // 31 tokens over 131072 and 65001 keys 223 us split, 194 us in pairs; a prompt of 200 tokens 11.3 and 16.4 us; 64 single tokens
   // over up to 8060 keys 69 and 89 us.
   const long long tiles = (static_cast<long long>(p.query_tokens) + p.tokens_per_tile - 1) / p.tokens_per_tile;
-  const bool pairs = tiles > p.batch && tiles * p.kv_heads * (most_keys / 128 + 1) >= 4ll * sm_count;
+  const long long keys = p.page_table != nullptr ? most_keys : most_keys / p.batch;
+  const bool pairs = tiles > p.batch && tiles * p.kv_heads * (keys / 128 + 1) >= 4ll * sm_count;
   SERVE_CUDA(launch_serve_attention(q_map, k_map, v_map, p, dtype, !pairs, sm_count, static_cast<cudaStream_t>(stream)));
   return FT_OK;
 }
@@ -667,7 +673,7 @@ int ft_prompt_attention_run(const ft_prompt_attention_args* a, void* workspace, 
   p.kv_heads = a->k.heads;
   p.head_dim = a->head_dim;
   p.causal = a->causal != 0;
-  return attention_run(p, a->q, a->out, maps[0], maps[1], a->dtype, a->key_tokens / a->batch, a->scale, workspace, workspace_bytes, status, sm_count, stream);
+  return attention_run(p, a->q, a->out, maps[0], maps[1], a->dtype, a->key_tokens, a->scale, workspace, workspace_bytes, status, sm_count, stream);
 }
 
 int ft_tree_attention_run(const ft_kv_cache* cache, const ft_tree_attention_args* a, void* workspace, size_t workspace_bytes, int* status,

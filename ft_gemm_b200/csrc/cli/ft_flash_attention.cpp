@@ -8,10 +8,14 @@
 // (N(0,1) by default, `--dist grid` for the reference's value grid), only the
 // score and output stages can be targeted, and verification covers
 // `--verify-rows` query rows spread over all heads (all rows when that many exist).
+// Beyond the reference's options: `--rotary` turns Q and K by their positions first,
+// `--unprotected` also runs the prompt attention of ft_serving.h on the same inputs,
+// which shows what the protection costs, and verifies it on the same rows.
 #include <cuda_fp16.h>
 
 #include "cli_common.h"
 #include "ft_attention.h"
+#include "ft_serving.h"
 
 static float half_bits_to_float(uint16_t h) {
   __half_raw raw;
@@ -95,6 +99,8 @@ int main(int argc, char** argv) {
   opt.softmax_rel_tol = args.get_float("--softmax-rel-tol", opt.softmax_rel_tol);
   opt.protect_softmax = args.has_flag("--protect-softmax") ? 1 : 0;
   opt.exact_prepare = args.has_flag("--exact-prepare") ? 1 : 0;
+  const bool rotary = args.has_flag("--rotary"), unprotected = args.has_flag("--unprotected");
+  const float rotary_base = args.get_float("--rotary-base", 10000.0f);
   if (args.has_flag("--help")) {
     std::printf(
         "Usage: %s [--batch N --heads N --sequence N --head-dim 64|128 --warmup N --repeat N --causal]\n"
@@ -102,7 +108,9 @@ int main(int argc, char** argv) {
         "       [--fault-stage none|score|softmax|softmax-state|output --fault-batch N --fault-head N --fault-query N --fault-index N --fault-value X]\n"
         "       [--fault2-query N --fault2-index N --fault2-value X]   (a second score fault in the same batch and head)\n"
         "       [--score-abs-tol X --score-rel-tol X --pv-abs-tol X --pv-rel-tol X]\n"
-        "       [--verify-abs-tol X --verify-rel-tol X --verify-rows N --dist normal|grid]\n",
+        "       [--verify-abs-tol X --verify-rel-tol X --verify-rows N --dist normal|grid]\n"
+        "       [--rotary --rotary-base X]   (rotary positions 0 .. N-1 for Q and K)\n"
+        "       [--unprotected]              (the prompt attention without checks, timed and verified beside it)\n",
         argv[0]);
     return EXIT_SUCCESS;
   }
@@ -144,6 +152,28 @@ int main(int argc, char** argv) {
   CLI_FT(ft_attention_generate_f16(d_v, count, 0x31415926U, dist_id, 1.0f, stream));
   CLI_CUDA(cudaStreamSynchronize(stream));
 
+  // [B, H, N, D] as N tokens of B * H heads
+  const ft_rows q_rows{d_q, head_dim, static_cast<long long>(sequence) * head_dim, batch * heads};
+  ft_rows k_rows = q_rows, v_rows = q_rows;
+  k_rows.data = d_k;
+  v_rows.data = d_v;
+  if (rotary) {
+    std::vector<long long> positions(sequence);
+    for (int i = 0; i < sequence; ++i) positions[i] = i;
+    long long* d_positions;
+    CLI_CUDA(cudaMalloc(reinterpret_cast<void**>(&d_positions), sequence * sizeof(long long)));
+    CLI_CUDA(cudaMemcpy(d_positions, positions.data(), sequence * sizeof(long long), cudaMemcpyHostToDevice));
+    ft_rotary_options rotary_options;
+    ft_rotary_options_default(&rotary_options, head_dim);
+    rotary_options.base = rotary_base;
+    ft_rotary_handle* rotary_handle = nullptr;
+    CLI_FT(ft_rotary_prepare(&rotary_handle, &rotary_options, stream));
+    CLI_FT(ft_rotary_run(rotary_handle, &q_rows, &q_rows, &k_rows, &k_rows, d_positions, sequence, FT_SRC_F16, 0, stream));
+    CLI_CUDA(cudaStreamSynchronize(stream));
+    CLI_FT(ft_rotary_destroy(rotary_handle));
+    CLI_CUDA(cudaFree(d_positions));
+  }
+
   // The metadata time reported is that of a second prepare: the first one also pays for loading the prepare kernels onto
   // the device (lazy module loading), which is not part of the operator's cost.
   ft_attn_handle* handle = nullptr;
@@ -175,13 +205,58 @@ int main(int argc, char** argv) {
   CLI_FT(ft_attention_fp16_abft_run(handle, d_out, stage == FT_ATTN_FAULT_NONE ? nullptr : &fault, stream));
   CLI_FT(ft_attention_fp16_abft_report(handle, &report));
 
+  // the same attention without checks: one sequence, every head its own
+  uint16_t* d_plain = nullptr;
+  float plain_ms = 0.0f;
+  if (unprotected) {
+    const int offsets[2] = {0, sequence};
+    int *d_offsets, *d_status;
+    void* d_workspace;
+    CLI_CUDA(cudaMalloc(reinterpret_cast<void**>(&d_plain), count * 2));
+    CLI_CUDA(cudaMalloc(reinterpret_cast<void**>(&d_offsets), sizeof(offsets)));
+    CLI_CUDA(cudaMalloc(reinterpret_cast<void**>(&d_status), sizeof(int)));
+    CLI_CUDA(cudaMalloc(&d_workspace, ft_attention_workspace()));
+    CLI_CUDA(cudaMemcpy(d_offsets, offsets, sizeof(offsets), cudaMemcpyHostToDevice));
+    CLI_CUDA(cudaMemset(d_status, 0, sizeof(int)));
+    ft_prompt_attention_args plain{};
+    plain.q = q_rows;
+    plain.k = k_rows;
+    plain.v = v_rows;
+    plain.out = q_rows;
+    plain.out.data = d_plain;
+    plain.q_offsets = d_offsets;
+    plain.batch = 1;
+    plain.query_tokens = plain.key_tokens = sequence;
+    plain.head_dim = head_dim;
+    plain.dtype = FT_SRC_F16;
+    plain.causal = causal ? 1 : 0;
+    for (int i = 0; i < warmup + 1; ++i) CLI_FT(ft_prompt_attention_run(&plain, d_workspace, ft_attention_workspace(), d_status, stream));
+    CLI_CUDA(cudaEventRecord(start, stream));
+    for (int i = 0; i < repeat; ++i) CLI_FT(ft_prompt_attention_run(&plain, d_workspace, ft_attention_workspace(), d_status, stream));
+    CLI_CUDA(cudaEventRecord(stop, stream));
+    CLI_CUDA(cudaEventSynchronize(stop));
+    CLI_CUDA(cudaEventElapsedTime(&plain_ms, start, stop));
+    plain_ms /= repeat;
+    int plain_status = 0;
+    CLI_CUDA(cudaMemcpy(&plain_status, d_status, sizeof(int), cudaMemcpyDeviceToHost));
+    if (plain_status != FT_OK) {
+      std::fprintf(stderr, "a device-side wait of the unprotected attention expired\n");
+      return EXIT_FAILURE;
+    }
+    CLI_CUDA(cudaFree(d_offsets));
+    CLI_CUDA(cudaFree(d_status));
+    CLI_CUDA(cudaFree(d_workspace));
+  }
+
   // FP64 verification of sampled query rows (the reference checks every row, a14:1203-1267)
   size_t total_rows = static_cast<size_t>(batch) * heads * sequence;
   size_t rows_to_check = std::min<size_t>(total_rows, static_cast<size_t>(verify_rows));
   float max_absolute_error = 0.0f, max_tolerance_ratio = 0.0f;
+  float plain_max_error = 0.0f;
   int mismatches = 0;
   std::vector<uint16_t> q_row(head_dim), k_head(static_cast<size_t>(sequence) * head_dim), v_head(k_head.size());
   std::vector<float> o_row(head_dim);
+  std::vector<uint16_t> plain_row(head_dim);
   std::vector<double> scores(sequence);
   long cached_head = -1;
   for (size_t s = 0; s < rows_to_check; ++s) {
@@ -195,6 +270,7 @@ int main(int argc, char** argv) {
     }
     CLI_CUDA(cudaMemcpy(q_row.data(), static_cast<uint16_t*>(d_q) + row * head_dim, head_dim * 2, cudaMemcpyDeviceToHost));
     CLI_CUDA(cudaMemcpy(o_row.data(), d_out + row * head_dim, head_dim * sizeof(float), cudaMemcpyDeviceToHost));
+    if (unprotected) CLI_CUDA(cudaMemcpy(plain_row.data(), d_plain + row * head_dim, head_dim * 2, cudaMemcpyDeviceToHost));
     const int key_count = causal ? static_cast<int>(row % sequence) + 1 : sequence;  // a14:1214
     double maximum = -1e300;
     for (int key = 0; key < key_count; ++key) {
@@ -217,6 +293,11 @@ int main(int argc, char** argv) {
       max_absolute_error = std::max(max_absolute_error, absolute_error);
       max_tolerance_ratio = std::max(max_tolerance_ratio, absolute_error / tolerance);
       mismatches += absolute_error > tolerance;
+      if (unprotected) {
+        const float plain_error = static_cast<float>(std::fabs(half_bits_to_float(plain_row[d]) - reference));
+        plain_max_error = std::max(plain_max_error, plain_error);
+        mismatches += plain_error > tolerance;
+      }
     }
   }
   bool fault_pass;
@@ -265,6 +346,13 @@ int main(int argc, char** argv) {
 #ifdef FT_ATTENTION_TRACE
   if (args.has_flag("--trace")) print_phase_trace(sequence / 128);
 #endif
+  if (rotary) std::printf("rotary_base: %.1f\n", rotary_base);
+  if (unprotected) {
+    std::printf("unprotected_time_ms: %.6f\n", plain_ms);
+    std::printf("unprotected_approx_attention_tflops: %.6f\n", attention_flops / (plain_ms * 1.0e9));
+    std::printf("unprotected_max_absolute_error: %.6e\n", plain_max_error);
+    CLI_CUDA(cudaFree(d_plain));
+  }
   std::printf("max_absolute_error: %.6e\n", max_absolute_error);
   std::printf("max_tolerance_ratio: %.6e\n", max_tolerance_ratio);
   std::printf("mismatches: %d\n", mismatches);

@@ -75,8 +75,8 @@ struct Layout {
   static constexpr int kTileBytes = kSlabs * 128 * 128;
   static constexpr int kQTiles = kSplitKeys ? 1 : 2;
   // What a row tile costs beside its key tiles, in key tiles (us at 1, 2, 3 and 4): 64 single tokens over up to 8060 keys 82, 70, 75, 79;
-  // ragged prompts in pairs 53.8, 55.4, 57.7, 60.2.
-  static constexpr int kItemCost = kSplitKeys ? 2 : 1;
+  // in pairs, ragged prompts with heads of 64 51.5, 53.3, 57.7, 60.2, 4 x 4096 tokens with heads of 128 513, 504, -, -.
+  static constexpr int kItemCost = kSplitKeys || kDim == 128 ? 2 : 1;
   static constexpr int kStages = kDim == 64 ? 10 : kSplitKeys ? 5 : 4;
   static constexpr int kBytes = (kQTiles + kStages) * kTileBytes + static_cast<int>(sizeof(Shared)) + 1024;
   static_assert(kBytes <= 232448 && kStages <= kMaxStages, "shared memory of one CTA");
@@ -330,13 +330,12 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   // ---- this CTA's share (warp 0): the lanes sum up the sequences' units, a stretch of sequences each
   Sequence seq = {};
   int first_sequence = 0;
-  long long left = 0, start = 0, share = 0, per_head = 1;  // units of the share; of it, in front in its sequence; per CTA; per key head
+  int left = 0, start = 0, share = 0, per_head = 1;  // units of the share; in front of it in its sequence; per CTA; per key head
   if (warp == 0) {
     const int per_lane = (p.batch + 31) / 32;
     const int scan_begin = min(lane * per_lane, p.batch), scan_end = min(scan_begin + per_lane, p.batch);
-    long long mine = 0, before = 0, share_begin = 0, at = 0;
+    int mine = 0, before = 0, share_begin = 0, at = 0, found = scan_begin;
     bool holds = false;
-    int found = scan_begin;
     // first the sums; then the lane whose stretch holds the beginning goes through it once more, unless it is one sequence
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
@@ -344,7 +343,7 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       for (int i = scan_begin; i < scan_end; ++i) {
         seq = load_sequence(p, i, tokens_per_item, L::kItemCost);
         per_head = seq.tiles.units_per_head();
-        const long long units = per_head * p.kv_heads;
+        const int units = per_head * p.kv_heads;
         if (pass == 0) {
           mine += units;
         } else {
@@ -357,14 +356,14 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       before = mine;  // inclusive prefix
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
-        const long long other = __shfl_up_sync(0xffffffffU, before, off);
+        const int other = __shfl_up_sync(0xffffffffU, before, off);
         if (lane >= off) before += other;
       }
-      const long long total = __shfl_sync(0xffffffffU, before, 31);
+      const int total = __shfl_sync(0xffffffffU, before, 31);
       before -= mine;
-      share = max(quotient(total + gridDim.x - 1, gridDim.x), static_cast<long long>(p.min_share));
-      share_begin = min(share * blockIdx.x, total);
-      left = min(share_begin + share, total) - share_begin;
+      share = max(total / static_cast<int>(gridDim.x) + 1, p.min_share);
+      share_begin = static_cast<int>(min(static_cast<long long>(share) * blockIdx.x, static_cast<long long>(total)));
+      left = min(share, total - share_begin);
       holds = left > 0 && before <= share_begin && share_begin < before + mine;
       at = before;
       if (!holds || per_lane == 1) break;
@@ -402,26 +401,26 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       bool ok = true;
       int kv_head = 0, row_tile = 0, first = 0;
       if (left > 0) {
-        kv_head = static_cast<int>(quotient(start, per_head));
-        const long long inner = start - kv_head * per_head;
-        int lo = 0;
-        long long in_front = 0;  // units_before(lo) <= inner
+        kv_head = start / per_head;
+        const int inner = start - kv_head * per_head;
+        int lo = 0, in_front = 0;  // units_before(lo) <= inner
         if (seq.tiles.ramp) {
+#pragma unroll 1
           for (int hi = seq.tiles.row_tiles; hi - lo > 1;) {
             const int step = (hi - lo + 31) / 32;
             const int probe = min(lo + lane * step, hi);
-            const long long units = seq.tiles.units_before(probe);
+            const int units = seq.tiles.units_before(probe);
             const int last = __popc(__ballot_sync(0xffffffffU, probe < hi && units <= inner)) - 1;
             in_front = __shfl_sync(0xffffffffU, units, last);
             lo = lo + last * step;
             hi = min(lo + step, hi);
           }
         } else {
-          lo = static_cast<int>(quotient(inner, seq.tiles.units_of(0)));
-          in_front = static_cast<long long>(lo) * seq.tiles.units_of(0);
+          lo = inner / seq.tiles.units_of(0);
+          in_front = lo * seq.tiles.units_of(0);
         }
         row_tile = lo;
-        first = static_cast<int>(inner - in_front);
+        first = inner - in_front;
         if (first <= L::kItemCost) {  // the whole row tile is this CTA's, whatever lies in front of the boundary
           left += first;
           first = 0;
@@ -442,7 +441,7 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           }
           break;
         }
-        const int end = static_cast<int>(min(static_cast<long long>(units), first + left));
+        const int end = min(units, first + left);
         item.place0 = row_tile * tokens_per_item;
         item.token0 = seq.token0 + item.place0;
         item.tokens = min(seq.tiles.queries - item.place0, tokens_per_item);
@@ -456,7 +455,7 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         item.slot = first == 0 && end == units ? -1 : first > 0 ? 0 : 1;
         if (first == 0 && end < units) {
           unfinished.valid = 1;
-          unfinished.last_cta = blockIdx.x + static_cast<int>(quotient(units - end + share - 1, share));
+          unfinished.last_cta = blockIdx.x + (units - end + share - 1) / share;
           unfinished.token0 = item.token0;
           unfinished.tokens = item.tokens;
           unfinished.kv_head = kv_head;
@@ -550,6 +549,8 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
               seq = make_sequence(p, next, tokens_per_item, L::kItemCost);
               next = load_raw(p, min(b + 1, p.batch - 1));
             } while (seq.tiles.row_tiles == 0 && b + 1 < p.batch);
+            // offsets that do not ascend may promise more than there is: nothing is read behind the last sequence
+            if (b >= p.batch || seq.tiles.row_tiles == 0) left = 0;
           }
         }
       }

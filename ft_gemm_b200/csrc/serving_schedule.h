@@ -11,39 +11,33 @@
 
 #ifdef __CUDACC__
 #define FT_HD __host__ __device__ __forceinline__
-#define FT_HD_CALL static __host__ __device__ __noinline__
 #else
 #define FT_HD inline
-#define FT_HD_CALL static inline
 #endif
 
 namespace ftg {
 
 constexpr int kKeyTile = 128;
 
-FT_HD_CALL long long wide_quotient(long long a, long long b) { return a / b; }
-// 64-bit numbers that nearly always fit into 32 bits, where a division is several times cheaper
-FT_HD long long quotient(long long a, long long b) {
-  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
-  return wide_quotient(a, b);
-}
+// All units of a call are numbered in 31 bits (the caller refuses more: at a microsecond each they would take seconds on
+// every SM of the device).
 
 // sum over i in [0, n) of floor((a i + b) / 128) for a, b >= 0.  The steps repeat every 128 / gcd(a, 128) terms with an
-// increment of a / gcd(a, 128): one period is added up term by term (at most 128 of them; at most 4 for the usual head groups), the
-// rest follows.
-FT_HD long long floor_sum(int n, int a, int b) {
+// increment of a / gcd(a, 128): one period is added up term by term (at most 128 of them; at most 4 for the usual head
+// groups), the rest follows.
+FT_HD int floor_sum(int n, int a, int b) {
   if (n <= 0) return 0;
   int shift = 0;  // period = 2^shift
   while (((a << shift) & (kKeyTile - 1)) != 0) ++shift;
   const int period = 1 << shift, step = (a << shift) / kKeyTile, periods = n >> shift, rest = n & (period - 1);
-  long long one = 0, head = 0;  // a whole period, and its first `rest` terms
+  int one = 0, head = 0;  // a whole period, and its first `rest` terms
   int at = b;
+#pragma unroll 1
   for (int i = 0; i < period; ++i, at += a) {
     if (i == rest) head = one;
     one += at / kKeyTile;
   }
-  return periods * one + static_cast<long long>(step) * period * (static_cast<long long>(periods) * (periods - 1) / 2) + head +
-         static_cast<long long>(rest) * periods * step;
+  return periods * one + step * period * static_cast<int>(static_cast<long long>(periods) * (periods - 1) / 2) + head + rest * periods * step;
 }
 
 struct SequenceTiles {
@@ -81,19 +75,19 @@ struct SequenceTiles {
     return tiles(limit(end < queries ? static_cast<int>(end) : queries)) + item_cost;
   }
   // units of the row tiles in front of r, r in [0, row_tiles]
-  FT_HD long long units_before(int r) const {
-    if (!ramp) return static_cast<long long>(r) * (tiles(keys) + item_cost);
+  FT_HD int units_before(int r) const {
+    if (!ramp) return r * (tiles(keys) + item_cost);
     const int inner = r < row_tiles ? r : row_tiles - 1;  // the last row tile ends with the queries, not on the line
     int empty = 0;                                        // row tiles that see nothing
     if (prefix < 0) {
       empty = -prefix / tokens_per_item;
       empty = empty > inner ? inner : empty;
     }
-    long long total = static_cast<long long>(inner) * item_cost + empty + floor_sum(inner - empty, tokens_per_item, tokens_per_item * (empty + 1) + prefix + kKeyTile - 1);
+    int total = inner * item_cost + empty + floor_sum(inner - empty, tokens_per_item, tokens_per_item * (empty + 1) + prefix + kKeyTile - 1);
     if (r == row_tiles && row_tiles > 0) total += units_of(row_tiles - 1);
     return total;
   }
-  FT_HD long long units_per_head() const { return row_tiles == 0 ? 0 : units_before(row_tiles); }
+  FT_HD int units_per_head() const { return row_tiles == 0 ? 0 : units_before(row_tiles); }
 };
 
 }  // namespace ftg

@@ -161,6 +161,49 @@ def test_python_refuses_what_is_not_a_cuda_cache(ftg):
         ftg.PromptAttention(8, 2, 128, dtype=torch.float32)
 
 
+SCHEDULE = r"""
+#include <cstdio>
+#include <cstdlib>
+#include "serving_schedule.h"
+using namespace ftg;
+// the units of a row tile, from the definition
+static int units(int n, int keys, int full, int per_item, int cost, bool chain, int r) {
+  const int end = (r + 1) * per_item < n ? (r + 1) * per_item : n;
+  int seen = chain && keys == full ? full - n + end : keys;  // keys that the tile's last row sees
+  if (seen < 1) seen = 1;
+  return (seen + 127) / 128 + cost;
+}
+int main() {
+  srand(7);
+  for (int i = 0; i < 30000; ++i) {
+    const int per_item = 1 + rand() % 256, n = rand() % (i % 3 ? 300 : 3000), full = i % 5 ? rand() % 3000 : rand() % 20;
+    const int keys = i % 7 == 0 && full ? rand() % full : full, cost = rand() % 4;
+    const bool chain = rand() % 3 != 0;
+    const SequenceTiles s = SequenceTiles::make(n, keys, full, per_item, cost, chain);
+    if (s.row_tiles != (n + per_item - 1) / per_item) return printf("row tiles\n"), 1;
+    int sum = 0;
+    for (int r = 0; r < s.row_tiles; ++r) {
+      if (s.units_before(r) != sum || s.units_of(r) != units(n, keys, full, per_item, cost, chain, r)) return printf("row tile %d of case %d\n", r, i), 1;
+      sum += s.units_of(r);
+    }
+    if (s.units_per_head() != sum) return printf("case %d\n", i), 1;
+  }
+  // the largest numbers: 2^30 keys
+  const SequenceTiles s = SequenceTiles::make(1, 1 << 30, 1 << 30, 32, 2, true);
+  return s.units_of(0) == (1 << 23) + 2 && s.units_per_head() == s.units_of(0) ? 0 : 1;
+}
+"""
+
+
+def test_shares_of_work_are_numbered_without_gaps(tmp_path):
+    """The closed forms that every CTA finds its share with, against counting (host build of the device code)."""
+    (tmp_path / "s.cpp").write_text(SCHEDULE)
+    subprocess.run(["g++", "-std=c++17", "-O2", "-fsanitize=undefined", "-fno-sanitize-recover", "-I", os.path.join(ROOT, "ft_gemm_b200", "csrc"),
+                    str(tmp_path / "s.cpp"), "-o", str(tmp_path / "s")], check=True)
+    out = subprocess.run([str(tmp_path / "s")], capture_output=True, text=True)
+    assert out.returncode == 0, out.stdout + out.stderr
+
+
 def test_tree_mask(ftg):
     pytest.importorskip("torch")
     rng = random.Random(3)

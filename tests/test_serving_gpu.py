@@ -11,6 +11,8 @@ Tolerances (u = eps/2 is the largest relative rounding error of the 16-bit type,
 * rotary: the angle's reduced form has a relative error of 2^-24, sine and cosine (2 units in the last place), their scaling,
   two products and a sum (3 more roundings): below 16 2^-24 (|a| + |b|) m in all; then one rounding, u |result|."""
 import math
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -582,6 +584,21 @@ def test_refusals(ftg):
     # nothing to do is no error
     op.run(x[:0], x[:0], x[:0], x[:0], offsets[:1])
     rotary.run(x[:0], None, torch.zeros(0, dtype=torch.int64, device="cuda"), x[:0])
+
+
+def test_attention_program_with_rotary_positions_and_without_protection(ftg):
+    """The command-line program rotates its inputs and runs the prompt attention beside the protected one; both are verified
+    in 64 bits on the same rows."""
+    exe = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "build", "ft_flash_attention")
+    if not os.path.exists(exe):
+        pytest.skip("the command-line programs are not built")
+    for extra in (["--causal", "--rotary"], ["--rotary", "--rotary-base", "500000", "--head-dim", "64", "--sequence", "333"], []):
+        out = subprocess.run([exe, *extra, "--batch", "2", "--heads", "3", "--sequence", "512", "--repeat", "2", "--verify-rows", "600", "--unprotected"],
+                             capture_output=True, text=True, timeout=300)
+        report = dict(line.split(": ", 1) for line in out.stdout.splitlines() if ": " in line)
+        assert out.returncode == 0 and report["verification"] == "PASS", out.stdout + out.stderr
+        assert float(report["unprotected_max_absolute_error"]) < 4e-3 and float(report["unprotected_time_ms"]) > 0
+        assert ("rotary_base" in report) == ("--rotary" in extra)
 
 
 def test_a_served_decoder_step_by_step(ftg):
