@@ -55,9 +55,9 @@ int check_cache(const ft_kv_cache* c) {
   if (c == nullptr || c->k == nullptr || c->v == nullptr) return noalloc_fail(FT_ERR_INVALID, "null cache, K or V");
   const int rc = check_dtype(c->dtype);
   if (rc != FT_OK) return rc;
-  if (c->layers <= 0 || c->layers > 32767 || c->pages <= 0 || c->kv_heads <= 0 || (c->head_dim != 64 && c->head_dim != 128)) {
-    return noalloc_fail(FT_ERR_INVALID, "the cache needs 1 to 32767 layers, pages, key heads and head_dim 64 or 128 (got %d, %d, %d, %d)", c->layers,
-                        c->pages, c->kv_heads, c->head_dim);
+  if (c->layers <= 0 || c->layers > 32767 || c->pages <= 0 || c->kv_heads <= 0 || c->kv_heads > 8192 || (c->head_dim != 64 && c->head_dim != 128)) {
+    return noalloc_fail(FT_ERR_INVALID, "the cache needs 1 to 32767 layers, pages, 1 to 8192 key heads and head_dim 64 or 128 (got %d, %d, %d, %d)",
+                        c->layers, c->pages, c->kv_heads, c->head_dim);
   }
   if (c->page_size < 8 || c->page_size > 256 || (c->page_size & (c->page_size - 1)) != 0) {
     return noalloc_fail(FT_ERR_INVALID, "page_size must be a power of two from 8 to 256 (got %d)", c->page_size);
@@ -251,6 +251,9 @@ int ft_rotary_prepare(ft_rotary_handle** handle, const ft_rotary_options* option
   return FT_OK;
 }
 
+// Rows of a block and blocks of a launch are counted in 31 bits.
+constexpr int kMaxRows = 1 << 30, kMaxHeads = 1 << 20;
+
 static void use_rotary(RotaryParams* p, const ft_rotary_handle* h) {
   p->turns = h->turns;
   p->rotary_dim = h->options.rotary_dim;
@@ -262,8 +265,9 @@ static void use_rotary(RotaryParams* p, const ft_rotary_handle* h) {
 int ft_rotary_run(const ft_rotary_handle* h, const ft_rows* q, const ft_rows* q_out, const ft_rows* k, const ft_rows* k_out, const long long* positions,
                   int tokens, int dtype, int inverse, void* stream) {
   if (h == nullptr || positions == nullptr) return noalloc_fail(FT_ERR_INVALID, "null handle or positions");
-  if (tokens < 0) return noalloc_fail(FT_ERR_INVALID, "negative token count");
+  if (tokens < 0 || tokens > kMaxRows) return noalloc_fail(FT_ERR_INVALID, "negative token count, or more than 2^30 tokens");
   if (q == nullptr || q->heads <= 0 || (k != nullptr && k->heads <= 0)) return noalloc_fail(FT_ERR_INVALID, "q needs at least one head, and k if given");
+  if (q->heads > kMaxHeads || (k != nullptr && k->heads > kMaxHeads)) return noalloc_fail(FT_ERR_INVALID, "q and k have at most %d heads", kMaxHeads);
   int rc = check_dtype(dtype);
   if (rc == FT_OK) rc = check_rows(q, "q", q->heads);
   if (rc == FT_OK) rc = check_rows(q_out, "q_out", q->heads);
@@ -295,7 +299,7 @@ int ft_kv_cache_append(const ft_kv_cache* cache, int layer, const ft_rows* k, co
   if (rc != FT_OK) return rc;
   if (layer < 0 || layer >= cache->layers) return noalloc_fail(FT_ERR_INVALID, "layer %d is outside the cache's %d", layer, cache->layers);
   if (slots == nullptr) return noalloc_fail(FT_ERR_INVALID, "null slots");
-  if (tokens < 0) return noalloc_fail(FT_ERR_INVALID, "negative token count");
+  if (tokens < 0 || tokens > kMaxRows) return noalloc_fail(FT_ERR_INVALID, "negative token count, or more than 2^30 tokens");
   rc = check_rows(k, "k", cache->kv_heads);
   if (rc == FT_OK) rc = check_rows(v, "v", cache->kv_heads);
   if (rc != FT_OK) return rc;
@@ -308,7 +312,7 @@ int ft_kv_cache_append(const ft_kv_cache* cache, int layer, const ft_rows* k, co
   p.head_dim = cache->head_dim;
   if (rotary != nullptr) use_rotary(&p, rotary);
   if (q != nullptr) {
-    if (q->heads <= 0) return noalloc_fail(FT_ERR_INVALID, "q needs at least one head");
+    if (q->heads <= 0 || q->heads > kMaxHeads) return noalloc_fail(FT_ERR_INVALID, "q needs 1 to %d heads", kMaxHeads);
     rc = check_rows(q, "q", q->heads);
     if (rc == FT_OK) rc = check_rows(q_out, "q_out", q->heads);
     if (rc != FT_OK) return rc;
@@ -336,8 +340,12 @@ int ft_kv_cache_append(const ft_kv_cache* cache, int layer, const ft_rows* k, co
 int ft_kv_cache_copy_pages(const ft_kv_cache* cache, const int* sources, const int* targets, int count, void* stream) {
   int rc = check_cache(cache);
   if (rc != FT_OK) return rc;
-  if (count < 0 || count > (1 << 24) || (count > 0 && (sources == nullptr || targets == nullptr))) {
-    return noalloc_fail(FT_ERR_INVALID, "copying pages needs 0 to 2^24 pairs with sources and targets (got %d)", count);
+  if (count < 0 || (count > 0 && (sources == nullptr || targets == nullptr))) {
+    return noalloc_fail(FT_ERR_INVALID, "copying pages needs pairs with sources and targets (got %d)", count);
+  }
+  if (count > copy_pages_most(cache->page_size * cache->kv_heads * cache->head_dim)) {  // blocks are counted in 31 bits
+    return noalloc_fail(FT_ERR_INVALID, "%d pages at once are too many: at most %d of this size", count,
+                        copy_pages_most(cache->page_size * cache->kv_heads * cache->head_dim));
   }
   CopyPagesParams p{};
   p.k = static_cast<uint16_t*>(cache->k);
@@ -575,7 +583,10 @@ size_t ft_attention_workspace(void) {
   return check_device(&sm_count) == FT_OK ? serve_attention_workspace(sm_count) : 0;
 }
 
-constexpr int kMaxTokens = 1 << 30;  // sums of a few of them stay inside 32 bits
+constexpr int kMaxQueries = 1 << 30;  // sums of a few of them stay inside 32 bits
+// A warp that has nothing to do for a row tile waits while the others go through its keys, and waits give up after 2
+// seconds: 2^20 key tiles take about one.
+constexpr int kMaxKeys = 1 << 27;
 
 static int check_heads(int heads, int kv_heads) {
   if (kv_heads <= 0 || heads <= 0 || heads % kv_heads != 0 || heads / kv_heads > 128) {
@@ -617,9 +628,9 @@ static int attention_run(ServeAttentionParams& p, const ft_rows& q, const ft_row
   p.status = status;
   // Two tiles of rows that go through the keys together halve what is read of K and V.  That needs sequences of more than
   // one tile, and enough key tiles for every SM; below that the finer items fill the SMs better.  (Only sizes that the
-  // host knows go into this: averages over the sequences, and the most keys there can be.)  B200, 32 heads of 128 on 8: trees of 64 and
-  // 31 tokens over 131072 and 65001 keys 223 us split, 194 us in pairs; a prompt of 200 tokens 11.3 and 16.4 us; 64 single tokens
-  // over up to 8060 keys 69 and 89 us.
+  // host knows go into this: averages over the sequences, and the most keys there can be.)  B200, 32 heads of 128 on 8: trees
+  // of 64 and 31 tokens over 131072 and 65001 keys 223 us split, 194 us in pairs; a prompt of 200 tokens 11.3 and 16.4 us; 64
+  // single tokens over up to 8060 keys 69 and 89 us.
   const long long tiles = (static_cast<long long>(p.query_tokens) + p.tokens_per_tile - 1) / p.tokens_per_tile;
   const long long keys = p.page_table != nullptr ? most_keys : most_keys / p.batch;
   const bool pairs = tiles > p.batch && tiles * p.kv_heads * (keys / 128 + 1) >= 4ll * sm_count;
@@ -635,8 +646,8 @@ int ft_prompt_attention_run(const ft_prompt_attention_args* a, void* workspace, 
   if (rc == FT_OK) rc = check_scale(a->scale);
   if (rc != FT_OK) return rc;
   if (a->head_dim != 64 && a->head_dim != 128) return noalloc_fail(FT_ERR_INVALID, "head_dim must be 64 or 128 (got %d)", a->head_dim);
-  if (a->batch < 0 || a->query_tokens < 0 || a->key_tokens < 0 || a->query_tokens > kMaxTokens || a->key_tokens > kMaxTokens) {
-    return noalloc_fail(FT_ERR_INVALID, "negative batch or token count, or more than 2^30 tokens");
+  if (a->batch < 0 || a->query_tokens < 0 || a->key_tokens < 0 || a->query_tokens > kMaxQueries || a->key_tokens > kMaxKeys) {
+    return noalloc_fail(FT_ERR_INVALID, "negative batch or token count, more than 2^30 queries or more than 2^27 keys");
   }
   if (a->batch == 0 || a->query_tokens == 0) return FT_OK;
   if (a->q_offsets == nullptr) return noalloc_fail(FT_ERR_INVALID, "null q_offsets");
@@ -685,11 +696,11 @@ int ft_tree_attention_run(const ft_kv_cache* cache, const ft_tree_attention_args
   if (rc == FT_OK) rc = check_scale(a->scale);
   if (rc != FT_OK) return rc;
   if (a->layer < 0 || a->layer >= cache->layers) return noalloc_fail(FT_ERR_INVALID, "layer %d is outside the cache's %d", a->layer, cache->layers);
-  if (a->batch < 0 || a->query_tokens < 0 || a->query_tokens > kMaxTokens) {
-    return noalloc_fail(FT_ERR_INVALID, "negative batch or token count, or more than 2^30 tokens");
+  if (a->batch < 0 || a->query_tokens < 0 || a->query_tokens > kMaxQueries) {
+    return noalloc_fail(FT_ERR_INVALID, "negative batch or token count, or more than 2^30 queries");
   }
-  if (a->table_pages <= 0 || a->table_stride < a->table_pages || a->table_pages > kMaxTokens / cache->page_size) {
-    return noalloc_fail(FT_ERR_INVALID, "the page table needs columns (at most 2^30 tokens) and a stride that holds them (got %d, %d)", a->table_pages,
+  if (a->table_pages <= 0 || a->table_stride < a->table_pages || a->table_pages > kMaxKeys / cache->page_size) {
+    return noalloc_fail(FT_ERR_INVALID, "the page table needs columns (at most 2^27 tokens) and a stride that holds them (got %d, %d)", a->table_pages,
                         a->table_stride);
   }
   if (a->mask != nullptr && (a->mask_words <= 0 || a->mask_stride < a->mask_words)) {
@@ -730,7 +741,8 @@ int ft_tree_attention_run(const ft_kv_cache* cache, const ft_tree_attention_args
   p.pages = cache->pages;
   p.table_pages = a->table_pages;
   p.table_stride = a->table_stride;
-  return attention_run(p, a->q, a->out, maps[0], maps[1], cache->dtype, static_cast<long long>(a->table_pages) * cache->page_size, a->scale, workspace, workspace_bytes, status, sm_count, stream);
+  return attention_run(p, a->q, a->out, maps[0], maps[1], cache->dtype, static_cast<long long>(a->table_pages) * cache->page_size, a->scale, workspace,
+                       workspace_bytes, status, sm_count, stream);
 }
 
 int ft_tree_mask(const int* parents, int nodes, uint32_t* mask, int words) {

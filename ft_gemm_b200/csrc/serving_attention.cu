@@ -11,13 +11,13 @@
 // probabilities go back to tensor memory in 16 bits over the scores they came from, and are the left operand of
 // O += P V.  A side has two warpgroups, one for each half of the 128 keys, so two threads share a row: one row per thread
 // leaves a scheduler with a single warp per side, whose latencies nothing hides (4 x 4096 tokens, 32 heads of 128: 570 us
-// against KSIDE us).  The exponent's reference follows the running maximum in steps of 2^8 only, so that the accumulator
+// against 505 us).  The exponent's reference follows the running maximum in steps of 2^8 only, so that the accumulator
 // in tensor memory is hardly ever rescaled; the two threads of a row exchange their maxima through shared memory.
 //
 //   warp 0      walks the share: item descriptors for the others, tensor copies of Q, K and V
 //   warp 1      one thread issues the matrix instructions
 //   warp 2      clears what lies behind the last key in the tile of V that holds it
-//   warps 3-6, 7-10, 11-14, 15-18   softmax of (A, first keys), (A, second), (B, first), (B, second), and what leaves the kernel
+//   warps 3-6, 7-10, 11-14, 15-18   softmax of (A, first keys), (A, second), (B, first), (B, second); they write the output too
 //
 // A share that begins or ends inside a row tile leaves its part (unnormalised O, reference and sum of each row) in the
 // workspace; serve_attention_combine_kernel adds the parts up.  Nothing depends on the order in which CTAs run.
@@ -35,9 +35,10 @@ namespace ftg {
 
 namespace {
 
-constexpr int kRows = 128;  // rows of a tile: the lanes of tensor memory
-constexpr int kRoleWarps = 3;                     // in front of the softmax warps
-constexpr int kThreads = (kRoleWarps + 16) * 32;  // 96 registers each: nothing spills in the loops, and spills go to an L1 cache that shared memory has left little of
+constexpr int kRows = 128;     // rows of a tile: the lanes of tensor memory
+constexpr int kRoleWarps = 3;  // in front of the softmax warps
+// 96 registers each.  Nothing spills in the loops: spills go to an L1 cache that shared memory has left little of.
+constexpr int kThreads = (kRoleWarps + 16) * 32;
 constexpr uint32_t kTimeoutNs = 2000000000u;
 constexpr float kRescaleStep = 8.0f;  // log2 units
 constexpr int kItems = 4;             // descriptors in flight
@@ -74,8 +75,9 @@ struct Layout {
   static constexpr int kSlabs = kDim / 64;              // 128-byte columns of a row of Q, K or V
   static constexpr int kTileBytes = kSlabs * 128 * 128;
   static constexpr int kQTiles = kSplitKeys ? 1 : 2;
-  // What a row tile costs beside its key tiles, in key tiles (us at 1, 2, 3 and 4): 64 single tokens over up to 8060 keys 82, 70, 75, 79;
-  // in pairs, ragged prompts with heads of 64 51.5, 53.3, 57.7, 60.2, 4 x 4096 tokens with heads of 128 513, 504, -, -.
+  // What a row tile costs beside its key tiles, in key tiles.  Split, 64 single tokens over up to 8060 keys take 82, 70, 75
+  // and 79 us at 1, 2, 3 and 4; in pairs, ragged prompts with heads of 64 take 51.5, 53.3, 57.7 and 60.2, 4 x 4096 tokens
+  // with heads of 128 513 and 504 at 1 and 2.
   static constexpr int kItemCost = kSplitKeys || kDim == 128 ? 2 : 1;
   static constexpr int kStages = kDim == 64 ? 10 : kSplitKeys ? 5 : 4;
   static constexpr int kBytes = (kQTiles + kStages) * kTileBytes + static_cast<int>(sizeof(Shared)) + 1024;
@@ -369,8 +371,10 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       if (!holds || per_lane == 1) break;
     }
     __syncwarp();
+    const unsigned holders = __ballot_sync(0xffffffffU, holds);
+    if (holders == 0) left = 0;
     if (left > 0) {
-      const int owner = __ffs(__ballot_sync(0xffffffffU, holds)) - 1;
+      const int owner = __ffs(holders) - 1;
       first_sequence = __shfl_sync(0xffffffffU, found, owner);
       start = share_begin - __shfl_sync(0xffffffffU, at, owner);
       per_head = __shfl_sync(0xffffffffU, per_head, owner);
@@ -384,6 +388,8 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       seq.tiles.item_cost = L::kItemCost;
       seq.tiles.chain = chain;
       seq.tiles.ramp = __shfl_sync(0xffffffffU, seq.tiles.ramp ? 1 : 0, owner) != 0;
+      // offsets that do not ascend can promise more than 31 bits of work: a share outside its sequence is left out
+      if (start < 0 || start / p.kv_heads >= per_head) left = 0;
     }
   }
   tcgen05_fence_before();
@@ -455,7 +461,7 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         item.slot = first == 0 && end == units ? -1 : first > 0 ? 0 : 1;
         if (first == 0 && end < units) {
           unfinished.valid = 1;
-          unfinished.last_cta = blockIdx.x + (units - end + share - 1) / share;
+          unfinished.last_cta = min(static_cast<int>(blockIdx.x) + (units - end + share - 1) / share, static_cast<int>(gridDim.x) - 1);
           unfinished.token0 = item.token0;
           unfinished.tokens = item.tokens;
           unfinished.kv_head = kv_head;
@@ -1010,7 +1016,12 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
 
 // Adds up the parts of the row tiles that were split over CTAs: block (c, y) takes the row tile that begins in CTA c and
 // does not end there.  A thread has four columns of one row; lanes run over rows first, as the parts are laid out.
-constexpr int kCombineBlocks = 8, kCombineThreads = 256;
+constexpr int kCombineThreads = 256;
+// Blocks per CTA.  Those of CTAs without such a row tile leave at once, but 148 x 8 of them cost about a microsecond; pairs have
+// twice the rows.  B200: trees over 131072 and 65001 tokens (pairs) 194.5 us with 8, 191.4 with 16, 190.7 with 24; a prompt of
+// 200 tokens (split) 10.9 with 4, 11.5 with 8, 12.7 with 16, one token over 1500 keys 12.9, 12.5 and 12.3.
+template <bool kSplitKeys>
+constexpr int kCombineBlocks = kSplitKeys ? 8 : 16;
 
 template <int kDim, bool kBf16>
 __global__ void __launch_bounds__(kCombineThreads) serve_attention_combine_kernel(const ServeAttentionParams p, int ctas, int halves) {
@@ -1024,7 +1035,7 @@ __global__ void __launch_bounds__(kCombineThreads) serve_attention_combine_kerne
   const int lane = threadIdx.x & 31;
   constexpr int kColumnGroups = kDim / 16;  // a warp takes 8 rows x 4 x 4 columns
   for (int unit = blockIdx.y * (kCombineThreads / 32) + threadIdx.x / 32; unit < halves * (kRows / 8) * kColumnGroups;
-       unit += kCombineBlocks * (kCombineThreads / 32)) {
+       unit += gridDim.y * (kCombineThreads / 32)) {
     const int columns = (unit % kColumnGroups) * 4 + (lane >> 3);
     const int rows = unit / kColumnGroups;
     const int half = rows / (kRows / 8), row = rows % (kRows / 8) * 8 + (lane & 7);
@@ -1087,7 +1098,7 @@ static cudaError_t launch_form(const CUtensorMap& q, const CUtensorMap& k, const
   config.numAttrs = 1;
   err = cudaLaunchKernelEx(&config, serve_attention_kernel<kDim, kBf16, kSplitKeys>, q, k, v, p);
   if (err != cudaSuccess) return err;
-  config.gridDim = dim3(sm_count, kCombineBlocks);
+  config.gridDim = dim3(sm_count, kCombineBlocks<kSplitKeys>);
   config.blockDim = dim3(kCombineThreads);
   config.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&config, serve_attention_combine_kernel<kDim, kBf16>, p, sm_count, static_cast<int>(L::kQTiles));

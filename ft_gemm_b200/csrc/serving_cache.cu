@@ -22,7 +22,6 @@ union Chunk {  // 16 bytes: eight elements
   T pairs[4];
 };
 
-
 // Rotates, copies and scatters the rows of `tokens_per_block` tokens.  A thread takes two 16-byte chunks of a row: the
 // two halves of eight pairs (or, interleaved, eight pairs outright), or two chunks that are only copied.  Sines and cosines
 // are computed once per token and frequency, shared by all heads, while the first rows are on their way: the angle in
@@ -228,9 +227,13 @@ cudaError_t launch_rotary(const RotaryParams& p, int dtype, cudaStream_t stream)
   return p.tokens <= 512 ? launch_rotary_threads<512>(p, dtype, 1, stream) : launch_rotary_threads<256>(p, dtype, p.tokens >= 4096 ? 2 : 1, stream);
 }
 
+static int pieces_of(int page_elements) { return (page_elements / 8 + kCopyThreads * kCopyUnroll - 1) / (kCopyThreads * kCopyUnroll); }
+
+int copy_pages_most(int page_elements) { return 0x7fffffff / pieces_of(page_elements); }
+
 cudaError_t launch_copy_pages(const CopyPagesParams& p, cudaStream_t stream) {
   if (p.count <= 0) return cudaSuccess;
-  const int pieces = (p.page_elements / 8 + kCopyThreads * kCopyUnroll - 1) / (kCopyThreads * kCopyUnroll);
+  const int pieces = pieces_of(p.page_elements);
   copy_pages_kernel<<<dim3(static_cast<unsigned>(p.count) * pieces, 2 * p.layers), kCopyThreads, 0, stream>>>(p, pieces);
   return cudaGetLastError();
 }

@@ -35,6 +35,7 @@ struct CopyPagesParams {
   int layers, pages, page_elements, count;
   const int *sources, *targets;
 };
+int copy_pages_most(int page_elements);  // pairs of one call
 cudaError_t launch_copy_pages(const CopyPagesParams& params, cudaStream_t stream);
 
 struct AcceptParams {

@@ -72,8 +72,9 @@ int ft_rotary_destroy(ft_rotary_handle* handle);
 
 /* Rotates q and k (k may be NULL) at positions[token].  An output may be its input
  * (the same data and strides); other overlaps are not allowed.  inverse != 0 turns
- * back, which is also the gradient: pass the output gradients as q and k.  Rows at or
- * behind `tokens` are neither read nor written. */
+ * back (times magnitude once more), which is also the gradient: pass the output gradients
+ * as q and k.  Rows at or behind `tokens` are neither read nor written.  At most 2^30
+ * tokens and 2^20 heads. */
 int ft_rotary_run(const ft_rotary_handle* handle, const ft_rows* q, const ft_rows* q_out, const ft_rows* k, const ft_rows* k_out,
                   const long long* positions, int tokens, int dtype, int inverse, void* stream);
 
@@ -89,7 +90,7 @@ typedef struct {
   long long layer_stride, page_stride, token_stride, head_stride;
   int layers, pages;
   int page_size; /* a power of two from 8 to 256 */
-  int kv_heads;
+  int kv_heads; /* at most 8192 */
   int head_dim; /* 64 or 128 */
   int dtype;
 } ft_kv_cache;
@@ -97,12 +98,14 @@ typedef struct {
 /* Writes k and v of `tokens` tokens to slots[token] = page * page_size + token in page of
  * one layer.  A token whose slot is negative or behind the last page is not written
  * (padding of a batch); the slots of one call must differ.  With `rotary`, k is rotated at
- * positions[token] on the way, and q (may be NULL) is rotated into q_out in the same pass. */
+ * positions[token] on the way, and q (may be NULL) is rotated into q_out in the same pass
+ * (q_out may be q). */
 int ft_kv_cache_append(const ft_kv_cache* cache, int layer, const ft_rows* k, const ft_rows* v, const long long* slots, int tokens,
                        const ft_rotary_handle* rotary, const long long* positions, const ft_rows* q, const ft_rows* q_out, void* stream);
 
 /* Copies page sources[i] to page targets[i] in every layer.  No target may be a source or
- * another target of the same call; pairs that name a page outside the cache are ignored. */
+ * another target of the same call; pairs that name a page outside the cache are ignored.  More
+ * than 2^31 - 1 pieces of 16 KiB in all (count times those of a page) are refused. */
 int ft_kv_cache_copy_pages(const ft_kv_cache* cache, const int* sources, const int* targets, int count, void* stream);
 
 /* Keeps the accepted ones of each sequence's drafted tokens: sequence b holds lengths[b]
@@ -110,8 +113,9 @@ int ft_kv_cache_copy_pages(const ft_kv_cache* cache, const int* sources, const i
  * token accepted[accepted_offsets[b] + i] (ascending in i) moves to place lengths[b] - n_b + i in
  * every layer, and new_lengths[b] (not the same array as lengths) becomes lengths[b] - n_b +
  * the number accepted.  page_table[b * table_stride + j] is the page of tokens
- * [j, j + 1) * page_size of sequence b, j < table_pages.  Moves that name a place outside the drafted tokens or
- * a page outside the cache are left out. */
+ * [j, j + 1) * page_size of sequence b, j < table_pages.  Offsets ascend, and the pages of the
+ * drafted tokens belong to one sequence only.  Moves that name a place outside the drafted tokens
+ * or a page outside the cache are left out. */
 int ft_kv_cache_accept(const ft_kv_cache* cache, const int* page_table, int table_pages, int table_stride, const int* lengths,
                        const int* drafted_offsets, const int* accepted, const int* accepted_offsets, int batch, int* new_lengths, void* stream);
 
@@ -119,7 +123,8 @@ int ft_kv_cache_accept(const ft_kv_cache* cache, const int* page_table, int tabl
  * Which sequence holds which page.  A forked sequence shares its pages with its parent
  * until one of them writes: _extend then gives the writer a copy of the last, partly
  * filled page.  Calls that move contents return the pairs to hand to
- * ft_kv_cache_copy_pages before the next append.  One thread at a time. */
+ * ft_kv_cache_copy_pages before the next append, and before _free or _truncate give a page
+ * back that one of the pairs names.  One thread at a time. */
 typedef struct ft_page_pool ft_page_pool;
 
 int ft_page_pool_create(ft_page_pool** pool, int pages, int page_size);
@@ -144,7 +149,13 @@ int ft_page_pool_compact(ft_page_pool* pool, int* host_sources, int* host_target
  * key head h / (heads / kv_heads), at most 128 query heads per key head.  A row that sees no
  * key gives zeros (and lse -inf).  head_dim is 64 or 128.  lse (may be NULL) is
  * float [token][head], the natural logarithm of the softmax denominator.  Output rows behind the
- * last sequence are left as they are.
+ * last sequence are left as they are.  `out` and lse overlap no input.  Packed k and v have at most
+ * 2^27 rows, a page table holds at most 2^27 tokens, and calls of more than some 2^31 tiles of 128
+ * rows by 128 keys are refused.
+ *
+ * What lies behind a sequence's last key never reaches its output, whatever it is.  A key that some
+ * rows of a sequence see and others do not has the probability zero in the others: K may hold
+ * anything there, but a NaN or an infinity in V can reach rows that do not see it (zero times V).
  *
  * `workspace` holds ft_attention_workspace() bytes, 16-byte aligned, contents arbitrary; calls that
  * can run at the same time need one each.  `status` is an int the caller sets to zero once; a

@@ -304,3 +304,35 @@ def test_page_pool_refusals(ftg, sv):
         pool.slots(s, 0, 1)
     with pytest.raises(ValueError):
         pool.extend([s], [1, 2])
+
+
+def test_sizes_that_a_launch_cannot_count_are_refused(sv, ftg):
+    lib = sv._lib()
+    # key heads beyond 8192: a page's elements would pass 31 bits
+    many = _cache(sv, kv_heads=8193, page_size=256, token_stride=8193 * 64, page_stride=256 * 8193 * 64)
+    assert lib.ft_kv_cache_copy_pages(many, None, None, 0, None) == ftg.FT_ERR_INVALID
+    # a page of 256 x 8192 x 128 elements is 32768 pieces of 16 KiB: 2^16 of them pass 2^31 - 1 blocks
+    large = _cache(sv, kv_heads=8192, page_size=256, head_dim=128, token_stride=8192 * 128, head_stride=128, page_stride=256 * 8192 * 128,
+                   layer_stride=1 << 40)
+    assert lib.ft_kv_cache_copy_pages(large, None, None, 0, None) == ftg.FT_OK
+    assert lib.ft_kv_cache_copy_pages(large, 0x1000, 0x2000, 1 << 16, None) == ftg.FT_ERR_INVALID
+    assert b"at most 65535" in lib.ft_gemm_last_error()
+    # rotary positions: 2^30 tokens, 2^20 heads
+    rows, rotary = sv.FtRows(0x1000, 64, 64, 1), 0x1000
+    wide = sv.FtRows(0x1000, 64, 0, (1 << 20) + 1)
+    assert lib.ft_rotary_run(rotary, rows, rows, None, None, 0x1000, (1 << 30) + 1, 1, 0, None) == ftg.FT_ERR_INVALID
+    assert lib.ft_rotary_run(rotary, wide, wide, None, None, 0x1000, 1, 1, 0, None) == ftg.FT_ERR_INVALID
+    assert lib.ft_rotary_run(rotary, rows, rows, wide, wide, 0x1000, 1, 1, 0, None) == ftg.FT_ERR_INVALID
+    good = sv.FtRows(0x1000, 128, 64, 2)
+    assert lib.ft_kv_cache_append(_cache(sv), 0, good, good, 0x1000, (1 << 30) + 1, None, None, None, None, None) == ftg.FT_ERR_INVALID
+    # attention: 2^27 keys, 2^30 queries
+    r = lambda heads: sv.FtRows(0x10000, heads * 128, 128, heads)  # noqa: E731
+    for queries, keys in ((16, (1 << 27) + 1), ((1 << 30) + 1, 16)):
+        a = sv.FtPromptAttentionArgs(r(8), r(2), r(2), r(8), None, 0x1000, 0x1000, 1, queries, keys, 128, 1, 1, 0.0)
+        assert lib.ft_prompt_attention_run(a, 0x100000, 1 << 40, 0x1000, None) == ftg.FT_ERR_INVALID
+        assert b"2^27 keys" in lib.ft_gemm_last_error()
+    x = sv.FtRows(0x10000, 4 * 64, 64, 4)
+    for pages in ((1 << 27) // 16 + 1, 2 ** 31 - 1):
+        a = sv.FtTreeAttentionArgs(x, x, None, 0x1000, 0x1000, 0x1000, None, 0, 0, 1, 4, pages, pages, 0, 0.0)
+        assert lib.ft_tree_attention_run(_cache(sv), a, 0x100000, 1 << 40, 0x1000, None) == ftg.FT_ERR_INVALID
+        assert b"2^27 tokens" in lib.ft_gemm_last_error()

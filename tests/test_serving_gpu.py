@@ -540,6 +540,156 @@ def test_streams_and_graphs(ftg):
     op.report(), tree.report()
 
 
+def test_a_call_with_more_tiles_than_it_can_number_is_refused(ftg):
+    """2^10 sequences of up to 2^24 keys with 32 key heads: refused before anything is launched."""
+    dtype = torch.bfloat16
+    cache = ftg.PagedCache.empty(1, 2, 256, 32, 64, dtype)
+    op, batch = ftg.TreeAttention(32, cache), 1 << 10
+    q = torch.zeros((batch, 32, 64), dtype=dtype, device="cuda")
+    table = torch.zeros((batch, 1 << 16), dtype=torch.int32, device="cuda")
+    held = torch.zeros(batch, dtype=torch.int32, device="cuda")
+    with pytest.raises(ftg.FtGemmError, match="too large"):
+        op.run(q, 0, torch.arange(batch + 1, dtype=torch.int32, device="cuda"), table, held, torch.empty_like(q))
+
+
+def test_a_captured_step_with_a_padded_batch(ftg):
+    """One decoding step of up to six sequences as a graph, replayed with fewer: the sequences that are not there have length
+    zero, no queries and negative slots.  Nothing of theirs is written, and the step's launches follow each other in the graph."""
+    gen, dtype, page, heads, kv_heads, d = _gen(30), torch.float16, 16, 6, 2, 128
+    cache = ftg.PagedCache.empty(2, 30, page, kv_heads, d, dtype)
+    cache.k.copy_(_randn(gen, cache.k.shape, dtype)), cache.v.copy_(_randn(gen, cache.v.shape, dtype))
+    rotary, tree = ftg.Rotary(d, rotary_dim=64), ftg.TreeAttention(heads, cache)
+    q, k, v = (_randn(gen, (6, h, d), dtype) for h in (heads, kv_heads, kv_heads))
+    q_out, out = torch.empty_like(q), torch.empty_like(q)
+    slots, positions = torch.full((6,), -1, device="cuda"), torch.zeros(6, dtype=torch.int64, device="cuda")
+    table = torch.full((6, 5), -1, dtype=torch.int32, device="cuda")
+    held, offsets = torch.zeros(6, dtype=torch.int32, device="cuda"), torch.zeros(7, dtype=torch.int32, device="cuda")
+
+    def step():
+        cache.append(1, k, v, slots, rotary=rotary, positions=positions, q=q, q_out=q_out)
+        tree.run(q_out, 1, offsets, table, held, out)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    pages = torch.randperm(30, generator=gen, device="cuda").to(torch.int32).view(6, 5).cpu()
+    for real in (6, 2, 0, 5):
+        lengths = [int(x) for x in np.random.RandomState(real).randint(1, 80, real)]
+        k.copy_(_randn(gen, k.shape, dtype)), v.copy_(_randn(gen, v.shape, dtype)), q.copy_(_randn(gen, q.shape, dtype))
+        k[real:], v[real:], q[real:] = math.nan, math.nan, math.nan
+        table.fill_(-1), slots.fill_(-1), positions.zero_(), held.zero_(), out.fill_(7.0)
+        for i, n in enumerate(lengths):
+            table[i] = pages[i]
+            slots[i] = int(pages[i, (n - 1) // page]) * page + (n - 1) % page
+            positions[i] = n - 1
+        held[:real] = torch.tensor(lengths, dtype=torch.int32)
+        offsets.copy_(torch.arange(7).clamp(max=real))
+        before = [x.clone() for x in (cache.k, cache.v)]
+        graph.replay()
+        tree.report()
+        turned = torch.empty_like(q), torch.empty_like(k)
+        rotary.run(q, k, positions, turned[0], turned[1])
+        for b, n in enumerate(lengths):
+            place = int(slots[b]) // page, int(slots[b]) % page
+            before[0][1, place[0], place[1]], before[1][1, place[0], place[1]] = turned[1][b], v[b]
+            kk, vv = (x[1, table[b].long()].reshape(-1, kv_heads, d)[:n] for x in before)
+            _check_rows(out[b:b + 1], None, turned[0][b:b + 1], kk, vv, torch.ones(1, n, dtype=torch.bool, device="cuda"), d ** -0.5)
+        assert torch.equal(before[0], cache.k) and torch.equal(before[1], cache.v)
+        assert bool((out[real:] == 7.0).all())
+
+
+def test_views_of_masks_and_tables(ftg):
+    """Rows of masks, page tables and lse of a wider buffer; masks with fewer bits than there are drafted tokens; two rows of the
+    table that name the same pages."""
+    gen, dtype, page, n, m = _gen(31), torch.bfloat16, 32, 40, 100
+    cache = ftg.PagedCache.empty(1, 8, page, 2, 64, dtype)
+    cache.k.copy_(_randn(gen, cache.k.shape, dtype)), cache.v.copy_(_randn(gen, cache.v.shape, dtype))
+    q = _randn(gen, (2 * n, 8, 64), dtype)
+    wide = torch.randint(-2 ** 31, 2 ** 31, (2 * n, 5), generator=gen, device="cuda").to(torch.int32)
+    tables = torch.tensor([[7, 5, 0, 3, 9, 9], [7, 5, 0, 3, 9, 9]], dtype=torch.int32, device="cuda")
+    out, op = torch.empty_like(q), ftg.TreeAttention(8, cache)
+    op.run(q, 0, _offsets([n, n]), tables[:, :4], torch.tensor([m, m], dtype=torch.int32, device="cuda"), out, mask=wide[:, 2:3])
+    op.report()
+    kk, vv = (x[0, tables[0, :4].long()].reshape(-1, 2, 64)[:m] for x in (cache.k, cache.v))
+    bits = (wide[:, 2:3] >> torch.arange(32, device="cuda")) & 1 == 1
+    for b in range(2):
+        rows = slice(b * n, b * n + n)
+        visible = torch.zeros((n, m), dtype=torch.bool, device="cuda")
+        visible[:, :m - n] = True
+        visible[:, m - n:m - n + 32] = bits[rows]  # the tokens behind the mask's 32 bits are seen by nobody
+        _check_rows(out[rows], None, q[rows], kk, vv, visible, 0.125)
+
+
+def test_keys_that_are_masked_may_hold_anything_in_k(ftg):
+    """NaN and infinities in K where a row does not see them, though other rows of the tile do."""
+    gen, dtype, n = _gen(32), torch.bfloat16, 150
+    q, k, v = (_randn(gen, (n, h, 64), dtype) for h in (4, 1, 1))
+    k[100], k[140] = math.nan, math.inf
+    out, op = torch.empty_like(q), ftg.PromptAttention(4, 1, 64, dtype=dtype)
+    op.run(q, k, v, out, _offsets([n]))
+    op.report()
+    clean = torch.where(k.isfinite(), k, torch.zeros_like(k))
+    _check_rows(out[:100], None, q[:100], clean, v, torch.ones(100, n, dtype=torch.bool, device="cuda").tril(), 0.125)
+    assert bool(out[100:].isnan().all())
+
+
+def test_page_operations_and_rotary_positions_in_graphs_and_on_streams(ftg):
+    gen, dtype = _gen(33), torch.bfloat16
+    cache = ftg.PagedCache.empty(2, 12, 8, 2, 64, dtype)
+    start = [_randn(gen, cache.k.shape, dtype) for _ in range(2)]
+    sources, targets = torch.tensor([3, 1, 3], dtype=torch.int32, device="cuda"), torch.tensor([5, 6, 7], dtype=torch.int32, device="cuda")
+    table = torch.tensor([[0, 2, 4], [9, 8, 10]], dtype=torch.int32, device="cuda")
+    held, drafted = torch.tensor([20, 9], dtype=torch.int32, device="cuda"), _offsets([9, 4])
+    accepted, ends, new = torch.tensor([0, 3, 8, 1, 3], dtype=torch.int32, device="cuda"), _offsets([3, 2]), torch.empty(2, dtype=torch.int32, device="cuda")
+    rotary, x = ftg.Rotary(64), _randn(gen, (5, 3, 64), dtype)
+    positions, twice = torch.arange(5, device="cuda") * 1000, torch.empty_like(x)
+
+    def calls(stream=None):
+        cache.copy_pages(sources, targets, stream=stream)
+        cache.accept(table, held, drafted, accepted, ends, new, stream=stream)
+        rotary.run(x, None, positions, twice, stream=stream)
+        rotary.run(twice, None, positions, twice, inverse=True, stream=stream)  # in place
+
+    results = []
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    for way in range(3):
+        cache.k.copy_(start[0]), cache.v.copy_(start[1]), new.zero_(), twice.zero_()
+        torch.cuda.synchronize()
+        if way == 0:
+            calls()
+        elif way == 1:
+            calls(side)
+        else:
+            with torch.cuda.graph(graph):
+                calls()
+            assert torch.equal(cache.k, start[0])  # captured only
+            graph.replay()
+        torch.cuda.synchronize()
+        results.append([y.clone() for y in (cache.k, cache.v, new, twice)])
+    for other in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(results[0], other))
+    want = [y.clone() for y in start]
+    for y in want:
+        y[:, [5, 6, 7]] = y[:, [3, 1, 3]]
+        for b, (n, own, kept) in enumerate(((20, 9, [0, 3, 8]), (9, 4, [1, 3]))):
+            flat = lambda i: (int(table[b, i // 8]), i % 8)  # noqa: E731
+            rows = [y[:, flat(n - own + j)[0], flat(n - own + j)[1]].clone() for j in kept]
+            for i, row in enumerate(rows):
+                y[:, flat(n - own + i)[0], flat(n - own + i)[1]] = row
+    assert torch.equal(results[0][0], want[0]) and torch.equal(results[0][1], want[1])
+    assert results[0][2].tolist() == [14, 7]
+    # there and back: two roundings of numbers that a rotation makes at most sqrt(2) times as large, and 2^-24-sized errors
+    pair = (x[..., :32].double() ** 2 + x[..., 32:].double() ** 2).sqrt()
+    off = (results[0][3].double() - x.double()).abs().amax(-1, keepdim=True)
+    bound = 1.02 * (2 * math.sqrt(2) * _half_eps(dtype)) * pair.amax(-1, keepdim=True) + 1e-30
+    assert bool((off <= bound).all())
+
+
 def test_refusals(ftg):
     dtype = torch.bfloat16
     x = torch.zeros((4, 2, 64), dtype=dtype, device="cuda")
