@@ -11,7 +11,7 @@
 // probabilities go back to tensor memory in 16 bits over the scores they came from, and are the left operand of
 // O += P V.  A side has two warpgroups, one for each half of the 128 keys, so two threads share a row: one row per thread
 // leaves a scheduler with a single warp per side, whose latencies nothing hides (4 x 4096 tokens, 32 heads of 128: 570 us
-// against 505 us).  The exponent's reference follows the running maximum in steps of 2^8 only, so that the accumulator
+// against 498 us).  The exponent's reference follows the running maximum in steps of 2^8 only, so that the accumulator
 // in tensor memory is hardly ever rescaled; the two threads of a row exchange their maxima through shared memory.
 //
 //   warp 0      walks the share: item descriptors for the others, tensor copies of Q, K and V
@@ -112,6 +112,22 @@ __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// The same on the FMA pipe: x = r + f with r a whole number (adding 1.5 * 2^23 rounds to it) and |f| <= 1/2; 2^f is the
+// polynomial of degree 5 with the smallest relative error there and a constant term of 1 (9.1e-8; fitted by least squares,
+// reweighted towards the largest errors until they level out), 2^r goes into the exponent bits.  At -127 and below the
+// result is 0, and a NaN stays one.
+__device__ __forceinline__ float exp2_polynomial(float x) {
+  float y;
+  asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(y) : "f"(x));
+  const float t = y + 12582912.0f;
+  const float f = y - (t - 12582912.0f);
+  float p = fmaf(0.00132647273f, f, 0.00967151299f);
+  p = fmaf(p, f, 0.0555073358f);
+  p = fmaf(p, f, 0.240222424f);
+  p = fmaf(p, f, 0.693147004f);
+  p = fmaf(p, f, 1.0f);
+  return p * __int_as_float((__float_as_int(t) << 23) + (127 << 23));
 }
 // Two numbers to 16 bits, the first in the low half.
 template <bool kBf16>
@@ -251,6 +267,16 @@ __device__ __forceinline__ Item load_item(const volatile Item& from) {
   i.end = from.end;
   i.slot = from.slot;
   return i;
+}
+
+// In pairs the unit for exponentials has as much to do as the tensor core (a tile's 128 x 128 take it 1024 cycles, the two
+// products with heads of 128 as many), so one exponential in eight goes to the FMA pipe: the pairs of numbers e of the
+// sixteen of a half.  B200, 4 x 4096 tokens, 32 heads, us without and with: heads of 64 849 -> 712 (causal 466 -> 390), heads of
+// 128 causal 508 -> 498.  Three pairs of sixteen: 815 and 525; one: 760 and 505; other places for two: 726 to 790 and 500 to 520.
+// One row tile waits for other things more: trees over up to 7700 keys 71.4 -> 72.7.
+template <int kDim, bool kSplitKeys>
+__device__ constexpr bool by_polynomial(int e) {
+  return !kSplitKeys && (e == 11 || e == (kDim == 64 ? 3 : 15));
 }
 
 // The queries of side `half` and the key tiles it works through.
@@ -853,8 +879,13 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             for (int e = 0; e < 16; ++e) {
               float lo, hi;
               unpack_f32x2(fma_f32x2(pack_f32x2(s[h * 32 + 2 * e], s[h * 32 + 2 * e + 1]), scale2, base2), lo, hi);
-              lo = exp2_approx(lo);
-              hi = exp2_approx(hi);
+              if (by_polynomial<kDim, kSplitKeys>(e)) {
+                lo = exp2_polynomial(lo);
+                hi = exp2_polynomial(hi);
+              } else {
+                lo = exp2_approx(lo);
+                hi = exp2_approx(hi);
+              }
               if (e & 1) {
                 sum_a = add_f32x2(sum_a, pack_f32x2(lo, hi));
               } else {

@@ -638,6 +638,41 @@ def test_keys_that_are_masked_may_hold_anything_in_k(ftg):
     assert bool(out[100:].isnan().all())
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("spread", [1.0, 12.0])
+def test_pairs_of_row_tiles(ftg, dim, dtype, spread):
+    """Enough rows and keys for two row tiles at a time, with scores close together and hundreds apart."""
+    gen, lengths, dtype = _gen(34), [1500, 3, 700, 257], DTYPES[dtype]
+    q, k, v = (_randn(gen, (sum(lengths), h, dim), dtype, s) for h, s in ((16, spread), (4, spread), (4, 1.0)))
+    for causal in (True, False):
+        out, lse = torch.empty_like(q), torch.empty((len(q), 16), device="cuda")
+        op = ftg.PromptAttention(16, 4, dim, dtype=dtype, causal=causal)
+        op.run(q, k, v, out, _offsets(lengths), lse=lse)
+        op.report()
+        at = 0
+        for n in lengths:
+            rows, visible = slice(at, at + n), torch.ones(n, n, dtype=torch.bool, device="cuda")
+            _check_rows(out[rows], lse[rows], q[rows], k[rows], v[rows], visible.tril() if causal else visible, dim ** -0.5)
+            at += n
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_nan_in_any_place_of_k_is_seen_by_the_rows_behind_it_only(ftg, dim):
+    """64 sequences with a NaN each, every place within 64 keys among them."""
+    gen, n, dtype = _gen(35), 400, torch.bfloat16
+    q, k, v = (_randn(gen, (64 * n, h, dim), dtype) for h in (4, 1, 1))
+    op, offsets, clean, out = ftg.PromptAttention(4, 1, dim, dtype=dtype), _offsets([n] * 64), torch.empty_like(q), torch.empty_like(q)
+    op.run(q, k, v, clean, offsets)
+    for j in range(64):
+        k[j * n + 300 + j] = math.nan
+    op.run(q, k, v, out, offsets)
+    op.report()
+    for j in range(64):
+        first = j * n + 300 + j
+        assert torch.equal(out[j * n:first], clean[j * n:first]) and bool(out[first:(j + 1) * n].isnan().all()), j
+
+
 def test_page_operations_and_rotary_positions_in_graphs_and_on_streams(ftg):
     gen, dtype = _gen(33), torch.bfloat16
     cache = ftg.PagedCache.empty(2, 12, 8, 2, 64, dtype)
