@@ -712,16 +712,24 @@ int ft_tree_attention_run(const ft_kv_cache* cache, const ft_tree_attention_args
   if (rc == FT_OK) rc = check_rows(&a->out, "out", a->q.heads);
   if (rc == FT_OK) rc = check_apart(&a->q, "q", a->query_tokens, cache->head_dim);
   if (rc == FT_OK) rc = check_apart(&a->out, "out", a->query_tokens, cache->head_dim);
+  if (rc != FT_OK) return rc;
+  // The copy engine sees groups of 8 tokens, numbered over all pages.
+  const long long page_groups = cache->page_stride / (8 * cache->token_stride);
+  const long long groups = (cache->pages - 1) * page_groups + cache->page_size / 8;
+  if (cache->page_stride % (8 * cache->token_stride) != 0 || (cache->pages + 1) * page_groups > INT32_MAX) {
+    return noalloc_fail(FT_ERR_INVALID, "the page stride (%lld) must be a multiple of that of 8 tokens (%lld), with fewer than 2^31 of them in the cache",
+                        cache->page_stride, 8 * cache->token_stride);
+  }
   int sm_count = 0;
-  if (rc == FT_OK) rc = check_device(&sm_count);
+  rc = check_device(&sm_count);
   if (rc != FT_OK) return rc;
   CUtensorMap maps[2];
   void* const kv[2] = {cache->k, cache->v};
   for (int i = 0; i < 2; ++i) {
-    const long long dims[4] = {cache->head_dim, cache->page_size, cache->kv_heads, cache->pages};
-    const long long strides[3] = {cache->token_stride, cache->head_stride, cache->page_stride};
-    const int boxes[4] = {64, std::min(cache->page_size, 128), 1, 1};
-    rc = make_map(&maps[i], cache->dtype, static_cast<const uint16_t*>(kv[i]) + a->layer * cache->layer_stride, 4, dims, strides, boxes);
+    const long long dims[5] = {64, 8, cache->head_dim / 64, groups, cache->kv_heads};
+    const long long strides[4] = {cache->token_stride, 64, 8 * cache->token_stride, cache->head_stride};
+    const int boxes[5] = {64, 8, cache->head_dim / 64, std::min(cache->page_size, 128) / 8, 1};
+    rc = make_map(&maps[i], cache->dtype, static_cast<const uint16_t*>(kv[i]) + a->layer * cache->layer_stride, 5, dims, strides, boxes);
     if (rc != FT_OK) return rc;
   }
   ServeAttentionParams p{};
@@ -738,6 +746,7 @@ int ft_tree_attention_run(const ft_kv_cache* cache, const ft_tree_attention_args
   p.head_dim = cache->head_dim;
   p.causal = 1;
   p.page_size = cache->page_size;
+  p.page_groups = static_cast<int>(page_groups);
   p.pages = cache->pages;
   p.table_pages = a->table_pages;
   p.table_stride = a->table_stride;

@@ -63,6 +63,7 @@ struct ServeAttentionParams {
   int heads, kv_heads, group, head_dim, causal;
   int tokens_per_tile;  // 128 / group: tokens whose heads fill a tile of 128 rows
   int page_size, pages, table_pages, table_stride;
+  int page_groups;   // groups of 8 tokens from page to page
   int min_share;     // key tiles that a CTA takes at least
   float scale_log2;  // log2(e) * scale
   void* workspace;
@@ -70,7 +71,7 @@ struct ServeAttentionParams {
 };
 size_t serve_attention_workspace(int sm_count);
 // q: [token][key head][head in group][d], boxes of 128 / group tokens; k, v: [token][key head][d] in boxes of 128 tokens, or
-// [page][key head][token in page][d] in boxes of up to 128 tokens of a page.  split_keys: one row tile per CTA, the two warpgroups
+// [key head][8 tokens][64 elements][token in 8][element] in boxes of up to 128 tokens of a page, the pages page_groups groups of 8 apart.  split_keys: one row tile per CTA, the two warpgroups
 // take turns on its key tiles.
 cudaError_t launch_serve_attention(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const ServeAttentionParams& params, int dtype,
                                    bool split_keys, int sm_count, cudaStream_t stream);

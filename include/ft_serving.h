@@ -83,7 +83,8 @@ int ft_rotary_run(const ft_rotary_handle* handle, const ft_rows* q, const ft_row
  * layer * layer_stride + page * page_stride + token * token_stride + head * head_stride + d.
  * Strides are in elements, multiples of 16 bytes, the same for K and V; a page of a
  * layer is dense in either order: (token_stride, head_stride) = (kv_heads * head_dim,
- * head_dim) or (head_dim, page_size * head_dim). */
+ * head_dim) or (head_dim, page_size * head_dim).  For the attention page_stride is a
+ * multiple of 8 * token_stride, as it is for dense pages and for pages of K and V in turn. */
 typedef struct {
   void* k;
   void* v;

@@ -336,3 +336,7 @@ def test_sizes_that_a_launch_cannot_count_are_refused(sv, ftg):
         a = sv.FtTreeAttentionArgs(x, x, None, 0x1000, 0x1000, 0x1000, None, 0, 0, 1, 4, pages, pages, 0, 0.0)
         assert lib.ft_tree_attention_run(_cache(sv), a, 0x100000, 1 << 40, 0x1000, None) == ftg.FT_ERR_INVALID
         assert b"2^27 tokens" in lib.ft_gemm_last_error()
+    # pages that do not begin on a group of 8 tokens
+    a = sv.FtTreeAttentionArgs(x, x, None, 0x1000, 0x1000, 0x1000, None, 0, 0, 1, 4, 4, 4, 0, 0.0)
+    assert lib.ft_tree_attention_run(_cache(sv, page_stride=16 * 2 * 64 + 64), a, 0x100000, 1 << 40, 0x1000, None) == ftg.FT_ERR_INVALID
+    assert b"page stride" in lib.ft_gemm_last_error()

@@ -638,6 +638,26 @@ def test_keys_that_are_masked_may_hold_anything_in_k(ftg):
     assert bool(out[100:].isnan().all())
 
 
+@pytest.mark.parametrize("page", [8, 16, 64, 256])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("by_head", [False, True])
+def test_pages_of_k_and_v_in_turn(ftg, page, dim, by_head):
+    """K and V of a page side by side in one buffer, the last page used, the one behind it named."""
+    gen, dtype, heads, pages, m = _gen(36), torch.bfloat16, 3, 9, 7 * page + 5
+    both = torch.full((2, pages, 2) + ((heads, page, dim) if by_head else (page, heads, dim)), math.nan, dtype=dtype, device="cuda")
+    k, v = (both[:, :, i].transpose(2, 3) if by_head else both[:, :, i] for i in range(2))
+    cache = ftg.PagedCache(k, v)
+    order = [8, 0, 3, 7, 1, 6, 2, 5]
+    plain = [_randn(gen, (m, heads, dim), dtype) for _ in range(2)]
+    cache.append(1, *plain, torch.tensor([order[i // page] * page + i % page for i in range(m)], device="cuda"))
+    q = _randn(gen, (3, 2 * heads, dim), dtype)
+    out, op = torch.empty_like(q), ftg.TreeAttention(2 * heads, cache)
+    op.run(q, 1, _offsets([3]), torch.tensor([order + [pages]], dtype=torch.int32, device="cuda"), torch.tensor([m], dtype=torch.int32, device="cuda"), out)
+    op.report()
+    visible = torch.arange(m, device="cuda")[None] <= torch.arange(3, device="cuda")[:, None] + m - 3
+    _check_rows(out, None, q, *plain, visible, dim ** -0.5)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("spread", [1.0, 12.0])
