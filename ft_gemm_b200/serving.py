@@ -51,6 +51,11 @@ _PACK_ROWS = struct.Struct(_ROWS).pack
 _PACK_PROMPT = struct.Struct(_ROWS * 4 + "PPPiiiiiif0P").pack
 _PACK_TREE = struct.Struct(_ROWS * 2 + "PPPPPiiiiiiif0P").pack
 
+# Looked up once: attribute chains cost as much as some of the calls.  (A torch without CUDA has none of them.)
+_get_device, _raw_stream, _raw_alloc, _raw_delete = (
+    getattr(torch._C, name, None) for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream", "_cuda_cudaCachingAllocator_raw_alloc",
+                                               "_cuda_cudaCachingAllocator_raw_delete"))
+
 _bound = False
 _calls = {}  # the entry points that run on a device, with structures given as packed bytes
 
@@ -99,7 +104,7 @@ def _lib():
 
 def _call(name: str, device: torch.device, *args):
     """One of _calls on the device of its tensors, which is nearly always the current one already."""
-    if torch._C._cuda_getDevice() == device.index:
+    if _get_device() == device.index:
         code = _calls[name](*args)
     else:
         with torch.cuda.device(device):
@@ -110,7 +115,7 @@ def _call(name: str, device: torch.device, *args):
 
 def _stream(device: torch.device, stream: Optional[torch.cuda.Stream]) -> int:
     if stream is None:
-        return torch._C._cuda_getCurrentRawStream(device.index)
+        return _raw_stream(device.index)
     if stream.device != device:
         raise ValueError(f"the stream belongs to {stream.device}, the tensors to {device}")
     return stream.cuda_stream
@@ -401,12 +406,19 @@ class _Attention:
             # the status word is zero before any other stream can run a kernel that writes to it
             torch.cuda.current_stream().synchronize()
 
-    def _workspace(self, stream: Optional[torch.cuda.Stream]) -> torch.Tensor:
-        """A workspace of this call's own, from the caller's allocator, on the stream that uses it."""
-        if stream is None:
-            return self.status.new_empty(self.workspace_bytes // 4)
-        with torch.cuda.stream(stream):
-            return self.status.new_empty(self.workspace_bytes // 4)
+    def _launch(self, name: str, device: torch.device, stream: int, *args):
+        """The call with a workspace of its own from torch's allocator, which belongs to `stream`: given back at once, it is used
+        again by what follows on that stream only.  (A tensor for it takes a microsecond longer.)"""
+        if _get_device() != device.index:
+            with torch.cuda.device(device):
+                return self._launch(name, device, stream, *args)
+        workspace = _raw_alloc(self.workspace_bytes, stream)
+        try:
+            code = _calls[name](*args, workspace, self.workspace_bytes, self.status_at, stream)
+        finally:
+            _raw_delete(workspace)
+        if code:
+            _abi.check(code)
 
     def report(self):
         """Waits for the device and raises if a device-side wait of an earlier run gave up: its output is not valid."""
@@ -443,8 +455,7 @@ class PromptAttention(_Attention):
         if batch <= 0 or tokens == 0:
             return
         args = _PACK_PROMPT(*rows, lse_at, at, key_at, batch, tokens, keys, head_dim, self.code, self.causal, self.scale)
-        workspace = self._workspace(stream)
-        _call("ft_prompt_attention_run", device, args, workspace.data_ptr(), self.workspace_bytes, self.status_at, _stream(device, stream))
+        self._launch("ft_prompt_attention_run", device, _stream(device, stream), args)
 
 
 class TreeAttention(_Attention):
@@ -472,8 +483,7 @@ class TreeAttention(_Attention):
         if batch <= 0 or tokens == 0:
             return
         args = _PACK_TREE(*rows, lse_at, at, table, held, mask_at, words, mask_stride, batch, tokens, columns, table_stride, layer, self.scale)
-        workspace = self._workspace(stream)
-        _call("ft_tree_attention_run", device, cache.address, args, workspace.data_ptr(), self.workspace_bytes, self.status_at, _stream(device, stream))
+        self._launch("ft_tree_attention_run", device, _stream(device, stream), cache.address, args)
 
 
 def _lse(lse: torch.Tensor, device: torch.device, tokens: int, heads: int) -> int:
