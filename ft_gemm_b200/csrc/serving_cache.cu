@@ -223,8 +223,14 @@ static cudaError_t launch_rotary_threads(const RotaryParams& p, int dtype, int t
 cudaError_t launch_rotary(const RotaryParams& p, int dtype, cudaStream_t stream) {
   if (p.tokens <= 0 || p.q_heads + p.k_heads + p.v_heads <= 0) return cudaSuccess;
   // Few tokens: a block of many threads per token, so that its rows go in one or two rounds (64 tokens: 2.4 us with 512 threads, 3.0
-  // with 256).  Many: smaller blocks, of two tokens once that fills the SMs (16384 tokens: 64 us, 72 with 512 threads).
-  return p.tokens <= 512 ? launch_rotary_threads<512>(p, dtype, 1, stream) : launch_rotary_threads<256>(p, dtype, p.tokens >= 4096 ? 2 : 1, stream);
+  // with 256).  Many: smaller blocks, of two tokens once that fills the SMs (16384 tokens: 64 us, 72 with 512 threads), or of
+  // three where a block's last round is then fuller (5001 tokens of 16 + 4 heads, 40 or 60 rows in two rounds of 32: 13.6 and
+  // 11.8 us; 16384 tokens of 32 + 8 + 8 heads, 96 rows in three rounds or 144 in five: 66.9 and 68.0).
+  if (p.tokens <= 512) return launch_rotary_threads<512>(p, dtype, 1, stream);
+  const int rows = p.q_heads + p.k_heads + p.v_heads, at_once = 256 / (p.head_dim / 16);
+  const int rounds_of_two = (2 * rows + at_once - 1) / at_once, rounds_of_three = (3 * rows + at_once - 1) / at_once;
+  const int tokens = p.tokens < 4096 ? 1 : 2 * rounds_of_three < 3 * rounds_of_two ? 3 : 2;
+  return launch_rotary_threads<256>(p, dtype, tokens, stream);
 }
 
 static int pieces_of(int page_elements) { return (page_elements / 8 + kCopyThreads * kCopyUnroll - 1) / (kCopyThreads * kCopyUnroll); }

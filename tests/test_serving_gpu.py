@@ -382,6 +382,33 @@ def test_rotary(ftg, case, dtype, inverse):
         assert torch.equal(fused[:, heads + kv_heads:], before[:, heads + kv_heads:]) and torch.equal(fused[tokens], before[tokens])
 
 
+@pytest.mark.parametrize("tokens,heads,kv_heads,d", [(513, 5, 2, 128), (2049, 12, 4, 64), (4096, 32, 8, 128), (4099, 16, 4, 128), (5000, 3, 1, 256),
+                                                      (4097, 24, 8, 64), (6001, 1, 1, 16)])
+def test_rotary_many_tokens(ftg, tokens, heads, kv_heads, d):
+    """Blocks of one, two and three tokens, the last one not full; with the append, q in place, rows of padding among them."""
+    gen, dtype = _gen(tokens), torch.bfloat16
+    rotary = ftg.Rotary(d)
+    q, k, v = (_randn(gen, (tokens, h, d), dtype) for h in (heads, kv_heads, kv_heads))
+    positions = torch.randint(0, 200_000, (tokens,), generator=gen, device="cuda")
+    q_out, k_out = torch.empty_like(q), torch.empty_like(k)
+    rotary.run(q, k, positions, q_out, k_out)
+    for x, y in ((q, q_out), (k, k_out)):
+        _check_rotated(y, *_rotated(x, positions, rotary.frequencies(), d, False, 1.0, False))
+    if d not in (64, 128):
+        return
+    pages = -(-tokens // 64) + 1
+    cache = ftg.PagedCache.empty(1, pages, 64, kv_heads, d, dtype)
+    cache.k.fill_(7.0), cache.v.fill_(7.0)
+    slots = torch.randperm(pages * 64, generator=gen, device="cuda")[:tokens]
+    slots[::10] = -1
+    cache.append(0, k, v, slots, rotary=rotary, positions=positions, q=q, q_out=q)
+    assert torch.equal(q, q_out)
+    for held, rows in ((cache.k, k_out), (cache.v, v)):
+        want = torch.full((pages * 64, kv_heads, d), 7.0, dtype=dtype, device="cuda")
+        want[slots[slots >= 0]] = rows[slots >= 0]
+        assert torch.equal(held.view(pages * 64, kv_heads, d), want)
+
+
 def test_rotary_inverse_is_the_gradient(ftg):
     """Against differences: a linear map's derivative along x is the map of x, so <g, R x> = <R^T g, x>, and R^T is `inverse`."""
     gen, n = _gen(3), 50
