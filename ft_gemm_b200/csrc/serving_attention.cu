@@ -884,6 +884,8 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
               }
             }
           }
+          // The probabilities are rounded to 16 bits once, as an operand of the second product; the denominator adds up the numbers
+          // before that, so that a row's roundings, of either sign, do not weigh on all of its values together.
           const float base = reference == -INFINITY ? 0.0f : reference;
           const unsigned long long scale2 = pack_f32x2(p.scale_log2, p.scale_log2), base2 = pack_f32x2(-base, -base);
           unsigned long long sum_a = pack_f32x2(sum, 0.0f), sum_b = pack_f32x2(0.0f, 0.0f);

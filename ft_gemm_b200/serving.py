@@ -294,7 +294,8 @@ class PagedCache:
 
 class PagePool:
     """Which sequence holds which page of a cache.  Forked sequences share pages until one of them writes to a page that it
-    shares; `extend` and `compact` move contents with the cache's copy_pages on `stream`."""
+    shares; `extend` and `compact` move contents with the cache's copy_pages on `stream`.  All of it is host work: a captured
+    step leaves it out, and takes the tables, lengths and slots that it gives from buffers filled before each replay."""
 
     def __init__(self, pages: int, page_size: int, cache: Optional[PagedCache] = None):
         if cache is not None and (cache.pages < pages or cache.page_size != page_size):
