@@ -75,9 +75,9 @@ struct Layout {
   static constexpr int kSlabs = kDim / 64;              // 128-byte columns of a row of Q, K or V
   static constexpr int kTileBytes = kSlabs * 128 * 128;
   static constexpr int kQTiles = kSplitKeys ? 1 : 2;
-  // What a row tile costs beside its key tiles, in key tiles.  Split, 64 single tokens over up to 8060 keys take 82, 70, 75
-  // and 79 us at 1, 2, 3 and 4; in pairs, ragged prompts with heads of 64 take 51.5, 53.3, 57.7 and 60.2, 4 x 4096 tokens
-  // with heads of 128 513 and 504 at 1 and 2.
+  // What a row tile costs beside its key tiles, in key tiles.  Split, 64 single tokens over up to 8060 keys take 89, 69, 75
+  // and 79 us at 1, 2, 3 and 4; in pairs, twenty ragged prompts with heads of 64 take 180, 190 and 202 at 1, 2 and 3, with
+  // heads of 128 and on fewer heads 123, 121 and 128.
   static constexpr int kItemCost = kSplitKeys || kDim == 128 ? 2 : 1;
   static constexpr int kStages = kDim == 64 ? 10 : kSplitKeys ? 5 : 4;
   static constexpr int kBytes = (kQTiles + kStages) * kTileBytes + static_cast<int>(sizeof(Shared)) + 1024;
