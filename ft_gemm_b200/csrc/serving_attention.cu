@@ -58,7 +58,7 @@ struct Item {
 struct Shared {
   uint64_t kv_full[kMaxStages], kv_empty[kMaxStages];
   uint64_t q_full, q_empty;
-  uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2];  // p_full: [side][first, second 64 keys]
+  uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
   uint64_t tail_wanted, tail_cleared;
   uint64_t item_full[kItems], item_empty[kItems];
   Item items[kItems];
@@ -344,8 +344,7 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     mbar_init(&sh.tail_cleared, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.p_full[i][0], 4);
-      mbar_init(&sh.p_full[i][1], 4);
+      mbar_init(&sh.p_full[i], 8);
       mbar_init(&sh.o_full[i], 1);
       mbar_init(&sh.o_empty[i], kSplitKeys ? 16 : 8);
       mbar_init(&sh.state_full[i], kSplitKeys ? 16 : 8);
@@ -664,23 +663,22 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             return (valid + 15) / 16;
           };
           // O += P V of side x for the key tile in v_stage, its i-th; the probabilities of its first 64 keys lie where their
-          // scores were, those of the others too
+          // scores were, those of the others too.  Each product adds to all columns of O, and when the reference moves each
+          // warpgroup rescales one half of them: even the products of the first 64 keys wait for both.  (B200, 4 x 4096
+          // tokens: 496 to 505 us, and 502 where the two warps of a row meet behind a rescale instead; ragged prompts 44 to 45 and 45.4.)
           auto accumulate = [&](int x, int i, int v_stage, int steps) -> bool {
             if (i == 0) {
               if (!wait(&sh.o_empty[x], o_phase[x] ^ 1)) return false;
               o_phase[x] ^= 1;
             }
             const uint32_t bd = v_desc + v_stage * (L::kTileBytes >> 4);
+            if (!wait(&sh.p_full[x], p_phase[x])) return false;
+            tcgen05_fence_after();
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (!wait(&sh.p_full[x][h], p_phase[x])) return false;
-              tcgen05_fence_after();
-#pragma unroll
-              for (int k = 4 * h; k < 4 * h + 4; ++k) {
-                if (k < steps) {
-                  umma_ts(tmem_base + kTmemO + x * kDim, tmem_base + kTmemS + x * 128 + h * 64 + (k % 4) * 8, bd + k * (rows.group >> 3), kv_high, kIdescO,
-                          i > 0 || k > 0);
-                }
+            for (int k = 0; k < 8; ++k) {
+              if (k < steps) {
+                umma_ts(tmem_base + kTmemO + x * kDim, tmem_base + kTmemS + x * 128 + (k / 4) * 64 + (k % 4) * 8, bd + k * (rows.group >> 3), kv_high, kIdescO,
+                        i > 0 || k > 0);
               }
             }
             p_phase[x] ^= 1;
@@ -919,7 +917,7 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         }
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.p_full[x][c]);
+        if (lane == 0) mbar_arrive(&sh.p_full[x]);
       }
       if (!ok) break;
 

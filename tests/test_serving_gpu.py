@@ -720,6 +720,51 @@ def test_a_nan_in_any_place_of_k_is_seen_by_the_rows_behind_it_only(ftg, dim):
         assert torch.equal(out[j * n:first], clean[j * n:first]) and bool(out[first:(j + 1) * n].isnan().all()), j
 
 
+def _climbing(gen, lengths, heads, kv_heads, dim, dtype):
+    """Queries of different sizes along one direction and, for each length, keys along it that grow from tile to tile: the
+    maxima of the rows rise by 2 to 14 powers of two with every 128 keys."""
+    t, keys = sum(n for n, _ in lengths), torch.cat([torch.arange(m, device="cuda") // 128 for _, m in lengths])
+    side = torch.randint(0, 2, (dim,), generator=gen, device="cuda") * 2.0 - 1.0
+    size = torch.rand((t, heads, 1), generator=gen, device="cuda") + 0.2
+    q = (side * size * (64 / dim) ** 0.5 + 0.1 * torch.randn((t, heads, dim), generator=gen, device="cuda")).to(dtype)
+    k = (side * keys[:, None, None] + 0.5 * torch.randn((len(keys), kv_heads, dim), generator=gen, device="cuda")).to(dtype)
+    return q, k, _randn(gen, (len(keys), kv_heads, dim), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", ["pairs", "split"])
+@pytest.mark.parametrize("paged", [False, True])
+def test_maxima_that_climb_from_tile_to_tile(ftg, paged, rows, dim, dtype):
+    """The accumulator is rescaled at nearly every tile, in both forms: right, and the same bits from run to run."""
+    gen, dtype, heads, kv_heads, page = _gen(40), DTYPES[dtype], 8, 2, 64
+    lengths = [(1, 2600 - 37 * i) for i in range(40)] if rows == "split" else [(260, 2500), (190, 1800), (500, 2100)]
+    q, k, v = _climbing(gen, lengths, heads, kv_heads, dim, dtype)
+    offsets, key_offsets = _offsets([n for n, _ in lengths]), _offsets([m for _, m in lengths])
+    out, again = torch.empty_like(q), torch.empty_like(q)
+    if paged:
+        held = [m for _, m in lengths]
+        pages, table = _paged(np.random.RandomState(40), held, page)
+        cache = ftg.PagedCache.empty(1, pages, page, kv_heads, dim, dtype)
+        cache.append(0, k, v, torch.tensor([int(table[b, i // page]) * page + i % page for b, m in enumerate(held) for i in range(m)], device="cuda"))
+        op = ftg.TreeAttention(heads, cache)
+        args = 0, offsets, torch.from_numpy(table).cuda(), torch.tensor(held, dtype=torch.int32, device="cuda")
+        run = lambda to: op.run(q, *args, to)  # noqa: E731
+    else:
+        op = ftg.PromptAttention(heads, kv_heads, dim, dtype=dtype)
+        run = lambda to: op.run(q, k, v, to, offsets, key_offsets=key_offsets)  # noqa: E731
+    run(out)
+    for _ in range(50):
+        run(again)
+        assert torch.equal(out, again)
+    op.report()
+    a = b = 0
+    for n, m in lengths:
+        visible = torch.arange(m, device="cuda")[None] <= torch.arange(n, device="cuda")[:, None] + (m - n)
+        _check_rows(out[a:a + n], None, q[a:a + n], k[b:b + m], v[b:b + m], visible, dim ** -0.5)
+        a, b = a + n, b + m
+
+
 def test_page_operations_and_rotary_positions_in_graphs_and_on_streams(ftg):
     gen, dtype = _gen(33), torch.bfloat16
     cache = ftg.PagedCache.empty(2, 12, 8, 2, 64, dtype)
