@@ -6,6 +6,7 @@
 #include <cmath>
 #include <cstring>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include "serving_kernels.h"
@@ -40,6 +41,33 @@ int check_rows(const ft_rows* r, const char* name, int heads) {
 int check_apart(const ft_rows* r, const char* name, int tokens, int head_dim) {
   if ((r->heads > 1 && r->head_stride < head_dim) || (tokens > 1 && r->token_stride < head_dim)) {
     return noalloc_fail(FT_ERR_INVALID, "the heads and tokens of %s must not share memory (strides %lld, %lld)", name, r->token_stride, r->head_stride);
+  }
+  return FT_OK;
+}
+
+// Do any two of the m * n blocks of `block` elements at i * a + j * b share memory?
+bool blocks_meet(long long a, long long m, long long b, long long n, long long block) {
+  if ((m > 1 && a < block) || (n > 1 && b < block)) return true;
+  if (m <= 1 || n <= 1 || (b - block) / a >= m - 1 || (a - block) / b >= n - 1) return false;  // one dimension lies within a step of the other
+  if (m > n) {
+    std::swap(a, b);
+    std::swap(m, n);
+  }
+  for (long long i = 1; i < m; ++i) {  // the two steps of b on either side of i * a
+    const __int128 at = static_cast<__int128>(i) * a, j = at / b, past = at - j * b;
+    if ((j >= 1 && j < n && past < block) || (j + 1 < n && b - past < block)) return true;
+  }
+  return false;
+}
+
+// Outputs are written by many threads at once: no two rows may share memory, and an output that is its input has its strides.
+int check_output(const ft_rows* r, const char* name, int tokens, int head_dim, const ft_rows* input) {
+  if (blocks_meet(r->head_stride, r->heads, r->token_stride, tokens, head_dim)) {
+    return noalloc_fail(FT_ERR_INVALID, "the heads and tokens of %s must not share memory (strides %lld, %lld)", name, r->token_stride, r->head_stride);
+  }
+  if (input != nullptr && r->data == input->data &&
+      ((r->heads > 1 && r->head_stride != input->head_stride) || (tokens > 1 && r->token_stride != input->token_stride))) {
+    return noalloc_fail(FT_ERR_INVALID, "%s lies where its input does, with other strides", name);
   }
   return FT_OK;
 }
@@ -273,6 +301,9 @@ int ft_rotary_run(const ft_rotary_handle* h, const ft_rows* q, const ft_rows* q_
   if (rc == FT_OK) rc = check_rows(q_out, "q_out", q->heads);
   if (rc == FT_OK && k != nullptr) rc = check_rows(k, "k", k->heads);
   if (rc == FT_OK && k != nullptr) rc = check_rows(k_out, "k_out", k->heads);
+  if (rc == FT_OK) rc = check_output(q_out, "q_out", tokens, h->options.head_dim, q);
+  if (rc == FT_OK && k != nullptr) rc = check_output(k_out, "k_out", tokens, h->options.head_dim, k);
+  if (rc == FT_OK && k != nullptr && q_out->data == k_out->data) rc = noalloc_fail(FT_ERR_INVALID, "q_out and k_out share memory");
   if (rc != FT_OK) return rc;
   RotaryParams p{};
   use_rotary(&p, h);
@@ -315,6 +346,7 @@ int ft_kv_cache_append(const ft_kv_cache* cache, int layer, const ft_rows* k, co
     if (q->heads <= 0 || q->heads > kMaxHeads) return noalloc_fail(FT_ERR_INVALID, "q needs 1 to %d heads", kMaxHeads);
     rc = check_rows(q, "q", q->heads);
     if (rc == FT_OK) rc = check_rows(q_out, "q_out", q->heads);
+    if (rc == FT_OK) rc = check_output(q_out, "q_out", tokens, cache->head_dim, q);
     if (rc != FT_OK) return rc;
     p.q = to_rows(q);
     p.q_out = to_rows(q_out);
@@ -654,7 +686,7 @@ int ft_prompt_attention_run(const ft_prompt_attention_args* a, void* workspace, 
   rc = check_rows(&a->q, "q", a->q.heads);
   if (rc == FT_OK) rc = check_rows(&a->out, "out", a->q.heads);
   if (rc == FT_OK) rc = check_apart(&a->q, "q", a->query_tokens, a->head_dim);
-  if (rc == FT_OK) rc = check_apart(&a->out, "out", a->query_tokens, a->head_dim);
+  if (rc == FT_OK) rc = check_output(&a->out, "out", a->query_tokens, a->head_dim, nullptr);
   if (rc == FT_OK && a->key_tokens > 0) {
     rc = check_rows(&a->k, "k", a->k.heads);
     if (rc == FT_OK) rc = check_rows(&a->v, "v", a->k.heads);
@@ -711,7 +743,7 @@ int ft_tree_attention_run(const ft_kv_cache* cache, const ft_tree_attention_args
   rc = check_rows(&a->q, "q", a->q.heads);
   if (rc == FT_OK) rc = check_rows(&a->out, "out", a->q.heads);
   if (rc == FT_OK) rc = check_apart(&a->q, "q", a->query_tokens, cache->head_dim);
-  if (rc == FT_OK) rc = check_apart(&a->out, "out", a->query_tokens, cache->head_dim);
+  if (rc == FT_OK) rc = check_output(&a->out, "out", a->query_tokens, cache->head_dim, nullptr);
   if (rc != FT_OK) return rc;
   // The copy engine sees groups of 8 tokens, numbered over all pages.
   const long long page_groups = cache->page_stride / (8 * cache->token_stride);

@@ -71,7 +71,8 @@ int ft_rotary_prepare(ft_rotary_handle** handle, const ft_rotary_options* option
 int ft_rotary_destroy(ft_rotary_handle* handle);
 
 /* Rotates q and k (k may be NULL) at positions[token].  An output may be its input
- * (the same data and strides); other overlaps are not allowed.  inverse != 0 turns
+ * (the same data and strides); other overlaps are not allowed, and the rows of an output must not share
+ * memory (inputs may: a broadcast head).  inverse != 0 turns
  * back (times magnitude once more), which is also the gradient: pass the output gradients
  * as q and k.  Rows at or behind `tokens` are neither read nor written.  At most 2^30
  * tokens and 2^20 heads. */
@@ -100,7 +101,7 @@ typedef struct {
  * one layer.  A token whose slot is negative or behind the last page is not written
  * (padding of a batch); the slots of one call must differ.  With `rotary`, k is rotated at
  * positions[token] on the way, and q (may be NULL) is rotated into q_out in the same pass
- * (q_out may be q). */
+ * (q_out may be q; its rows must not share memory). */
 int ft_kv_cache_append(const ft_kv_cache* cache, int layer, const ft_rows* k, const ft_rows* v, const long long* slots, int tokens,
                        const ft_rotary_handle* rotary, const long long* positions, const ft_rows* q, const ft_rows* q_out, void* stream);
 

@@ -340,3 +340,55 @@ def test_sizes_that_a_launch_cannot_count_are_refused(sv, ftg):
     a = sv.FtTreeAttentionArgs(x, x, None, 0x1000, 0x1000, 0x1000, None, 0, 0, 1, 4, 4, 4, 0, 0.0)
     assert lib.ft_tree_attention_run(_cache(sv, page_stride=16 * 2 * 64 + 64), a, 0x100000, 1 << 40, 0x1000, None) == ftg.FT_ERR_INVALID
     assert b"page stride" in lib.ft_gemm_last_error()
+
+
+class _Handle(ctypes.Structure):
+    """A rotary handle as the library lays it out, for calls that are refused before they look at the frequencies."""
+
+
+def _handle(sv, head_dim):
+    if not hasattr(_Handle, "_fields_"):
+        _Handle._fields_ = [("options", sv.FtRotaryOptions), ("turns", ctypes.c_void_p)]
+    h = _Handle()
+    sv._lib().ft_rotary_options_default(ctypes.byref(h.options), head_dim)
+    return h
+
+
+def _share(strides, counts, block):
+    """Do two blocks at i * strides[0] + j * strides[1] share an element?"""
+    at = sorted(i * strides[0] + j * strides[1] for i in range(counts[0]) for j in range(counts[1]))
+    return any(b - a < block for a, b in zip(at, at[1:]))
+
+
+def test_outputs_whose_rows_share_memory_are_refused(sv, ftg):
+    """Expanded outputs, and all others in which two rows meet, from the definition; what is refused never reaches a device."""
+    lib, rng, refused = sv._lib(), random.Random(5), 0
+    shapes = [((0, 64), (4, 2)), ((64, 64), (4, 2)), ((128, 0), (4, 2)), ((64, 128), (4, 2)), ((32, 256), (4, 2))]
+    for _ in range(3000):
+        shapes.append(((8 * rng.randint(0, 40), 8 * rng.randint(0, 40)), (rng.randint(1, 9), rng.randint(1, 9))))
+    h = _handle(sv, 64)
+    for (token, head), (tokens, heads) in shapes:
+        if not _share((token, head), (tokens, heads), 64):
+            continue
+        refused += 1
+        fine, bad = sv.FtRows(0x100000, heads * 64, 64, heads), sv.FtRows(0x200000, token, head, heads)
+        for q_out, k, k_out in ((bad, None, None), (fine, fine, bad)):
+            q = sv.FtRows(0x300000, heads * 64, 64, heads)
+            assert lib.ft_rotary_run(ctypes.byref(h), q, q_out, k, k_out, 0x1000, tokens, 1, 0, None) == ftg.FT_ERR_INVALID
+            assert b"share memory" in lib.ft_gemm_last_error()
+        kv = sv.FtRows(0x100000, 128, 64, 2)
+        assert lib.ft_kv_cache_append(_cache(sv), 0, kv, kv, 0x1000, tokens, ctypes.byref(h), 0x1000, fine, bad, None) == ftg.FT_ERR_INVALID
+        assert b"share memory" in lib.ft_gemm_last_error()
+        kv = sv.FtRows(0x100000, 64, 64, 1)
+        a = sv.FtPromptAttentionArgs(fine, kv, kv, bad, None, 0x1000, None, 1, tokens, tokens, 64, 1, 1, 0.0)
+        assert lib.ft_prompt_attention_run(a, 0x100000, 1 << 40, 0x1000, None) == ftg.FT_ERR_INVALID
+        assert b"share memory" in lib.ft_gemm_last_error()
+        cache = _cache(sv, kv_heads=1, token_stride=64)
+        t = sv.FtTreeAttentionArgs(fine, bad, None, 0x1000, 0x1000, 0x1000, None, 0, 0, 1, tokens, 4, 4, 0, 0.0)
+        assert lib.ft_tree_attention_run(cache, t, 0x100000, 1 << 40, 0x1000, None) == ftg.FT_ERR_INVALID
+        assert b"share memory" in lib.ft_gemm_last_error()
+    assert refused > 500
+    # in place with other strides, and Q and K into one place
+    q = sv.FtRows(0x300000, 128, 64, 2)
+    assert lib.ft_rotary_run(ctypes.byref(h), q, sv.FtRows(0x300000, 64, 4 * 64, 2), None, None, 0x1000, 4, 1, 0, None) == ftg.FT_ERR_INVALID
+    assert lib.ft_rotary_run(ctypes.byref(h), q, sv.FtRows(0x400000, 128, 64, 2), q, sv.FtRows(0x400000, 128, 64, 2), 0x1000, 4, 1, 0, None) == ftg.FT_ERR_INVALID

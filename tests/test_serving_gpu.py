@@ -765,6 +765,28 @@ def test_maxima_that_climb_from_tile_to_tile(ftg, paged, rows, dim, dtype):
         a, b = a + n, b + m
 
 
+@pytest.mark.parametrize("strides", [(640, 128, 3), (128, 1280, 3), (1024, 384, 2), (384, 1024, 3)])
+def test_outputs_in_any_layout_whose_rows_are_apart(ftg, strides):
+    """By token, by head, and with tokens and heads between each other; broadcast inputs."""
+    token, head, heads = strides
+    gen, dtype, n, d = _gen(41), torch.bfloat16, 2 if (token, head) == (1024, 384) else 7, 128
+    room = torch.full(((n - 1) * token + (heads - 1) * head + d,), 7.0, dtype=dtype, device="cuda")
+    out, want = room.as_strided((n, heads, d), (token, head, 1)), torch.empty((n, heads, d), dtype=dtype, device="cuda")
+    one, positions = _randn(gen, (n, 1, d), dtype).expand(n, heads, d), torch.arange(n, device="cuda") * 77
+    rotary = ftg.Rotary(d)
+    rotary.run(one, None, positions, want)
+    rotary.run(one, None, positions, out)
+    assert torch.equal(out, want) and int((room != 7.0).sum()) <= out.numel()
+    with pytest.raises(ftg.FtGemmError, match="share memory"):
+        rotary.run(one, None, positions, one)
+    q, k = _randn(gen, (n, heads, d), dtype), _randn(gen, (n, 1, d), dtype)
+    op = ftg.PromptAttention(heads, 1, d, dtype=dtype)
+    op.run(q, k, k, want, _offsets([n]))
+    op.run(q, k, k, out, _offsets([n]))
+    op.report()
+    assert torch.equal(out, want)
+
+
 def test_page_operations_and_rotary_positions_in_graphs_and_on_streams(ftg):
     gen, dtype = _gen(33), torch.bfloat16
     cache = ftg.PagedCache.empty(2, 12, 8, 2, 64, dtype)
