@@ -101,6 +101,11 @@ int check_cache(const ft_kv_cache* c) {
       c->layer_stride < 0) {
     return noalloc_fail(FT_ERR_INVALID, "K and V must be 16-byte aligned, with page and layer strides that are multiples of 8 elements, and pages must not overlap");
   }
+  // accept moves rows of all layers at once
+  if (blocks_meet(c->page_stride, c->pages, c->layer_stride, c->layers, c->page_size * c->kv_heads * d)) {
+    return noalloc_fail(FT_ERR_INVALID, "the pages of different layers must not share memory (layer stride %lld, page stride %lld)", c->layer_stride,
+                        c->page_stride);
+  }
   return FT_OK;
 }
 
@@ -303,7 +308,7 @@ int ft_rotary_run(const ft_rotary_handle* h, const ft_rows* q, const ft_rows* q_
   if (rc == FT_OK && k != nullptr) rc = check_rows(k_out, "k_out", k->heads);
   if (rc == FT_OK) rc = check_output(q_out, "q_out", tokens, h->options.head_dim, q);
   if (rc == FT_OK && k != nullptr) rc = check_output(k_out, "k_out", tokens, h->options.head_dim, k);
-  if (rc == FT_OK && k != nullptr && q_out->data == k_out->data) rc = noalloc_fail(FT_ERR_INVALID, "q_out and k_out share memory");
+  if (rc == FT_OK && k != nullptr && tokens > 0 && q_out->data == k_out->data) rc = noalloc_fail(FT_ERR_INVALID, "q_out and k_out share memory");
   if (rc != FT_OK) return rc;
   RotaryParams p{};
   use_rotary(&p, h);

@@ -82,8 +82,8 @@ int ft_rotary_run(const ft_rotary_handle* handle, const ft_rows* q, const ft_row
 /* ---- paged key/value cache -------------------------------------------------------
  * K and V of `layers` layers: element (layer, page, token in page, head, d) lies at
  * layer * layer_stride + page * page_stride + token * token_stride + head * head_stride + d.
- * Strides are in elements, multiples of 16 bytes, the same for K and V; a page of a
- * layer is dense in either order: (token_stride, head_stride) = (kv_heads * head_dim,
+ * Strides are in elements, multiples of 16 bytes, the same for K and V; no two pages of
+ * any layers share memory (layers may lie between pages); a page of a layer is dense in either order: (token_stride, head_stride) = (kv_heads * head_dim,
  * head_dim) or (head_dim, page_size * head_dim).  For the attention page_stride is a
  * multiple of 8 * token_stride, as it is for dense pages and for pages of K and V in turn. */
 typedef struct {

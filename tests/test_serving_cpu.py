@@ -392,3 +392,18 @@ def test_outputs_whose_rows_share_memory_are_refused(sv, ftg):
     q = sv.FtRows(0x300000, 128, 64, 2)
     assert lib.ft_rotary_run(ctypes.byref(h), q, sv.FtRows(0x300000, 64, 4 * 64, 2), None, None, 0x1000, 4, 1, 0, None) == ftg.FT_ERR_INVALID
     assert lib.ft_rotary_run(ctypes.byref(h), q, sv.FtRows(0x400000, 128, 64, 2), q, sv.FtRows(0x400000, 128, 64, 2), 0x1000, 4, 1, 0, None) == ftg.FT_ERR_INVALID
+
+
+def test_layers_that_share_memory_are_refused(sv, ftg):
+    """Against the definition; pages of one layer between those of another are fine where they do not meet."""
+    lib, rng, page, seen = sv._lib(), random.Random(6), 16 * 2 * 64, {True: 0, False: 0}
+    cases = [(0, page, 2, 4), (page, page, 2, 4), (3 * page, page, 2, 4), (4 * page, page, 2, 4), (page, 2 * page, 2, 4), (page, 2 * page, 3, 4),
+             (page // 2, 2 * page, 2, 1), (0, page, 1, 4), (0, page, 3, 1)]
+    for _ in range(2000):
+        cases.append((page // 8 * rng.randint(0, 70), page // 8 * rng.randint(8, 70), rng.randint(1, 7), rng.randint(1, 7)))
+    for layer_stride, page_stride, layers, pages in cases:
+        meet = _share((layer_stride, page_stride), (layers, pages), page)
+        cache = _cache(sv, layer_stride=layer_stride, page_stride=page_stride, layers=layers, pages=pages)
+        assert (lib.ft_kv_cache_copy_pages(cache, None, None, 0, None) == ftg.FT_ERR_INVALID) == meet, (layer_stride, page_stride, layers, pages)
+        seen[meet] += 1
+    assert min(seen.values()) > 300
