@@ -109,6 +109,13 @@ int check_cache(const ft_kv_cache* c) {
   return FT_OK;
 }
 
+// Calls that write rows of K and rows of V at the same time.
+int check_two_slabs(const ft_kv_cache* c) {
+  const int rc = check_cache(c);
+  if (rc == FT_OK && c->k == c->v) return noalloc_fail(FT_ERR_INVALID, "K and V of the cache are the same memory: only reading and copying pages work there");
+  return rc;
+}
+
 int check_scale(float scale) {
   if (!(scale >= 0.0f) || !std::isfinite(scale)) return noalloc_fail(FT_ERR_INVALID, "scale must be positive and finite (0: 1 / sqrt(head_dim))");
   return FT_OK;
@@ -331,7 +338,7 @@ int ft_rotary_run(const ft_rotary_handle* h, const ft_rows* q, const ft_rows* q_
 
 int ft_kv_cache_append(const ft_kv_cache* cache, int layer, const ft_rows* k, const ft_rows* v, const long long* slots, int tokens,
                        const ft_rotary_handle* rotary, const long long* positions, const ft_rows* q, const ft_rows* q_out, void* stream) {
-  int rc = check_cache(cache);
+  int rc = check_two_slabs(cache);
   if (rc != FT_OK) return rc;
   if (layer < 0 || layer >= cache->layers) return noalloc_fail(FT_ERR_INVALID, "layer %d is outside the cache's %d", layer, cache->layers);
   if (slots == nullptr) return noalloc_fail(FT_ERR_INVALID, "null slots");
@@ -401,7 +408,7 @@ int ft_kv_cache_copy_pages(const ft_kv_cache* cache, const int* sources, const i
 
 int ft_kv_cache_accept(const ft_kv_cache* cache, const int* page_table, int table_pages, int table_stride, const int* lengths,
                        const int* drafted_offsets, const int* accepted, const int* accepted_offsets, int batch, int* new_lengths, void* stream) {
-  int rc = check_cache(cache);
+  int rc = check_two_slabs(cache);
   if (rc != FT_OK) return rc;
   if (batch < 0 || table_pages <= 0 || table_stride < table_pages) {
     return noalloc_fail(FT_ERR_INVALID, "batch must not be negative, the page table needs columns and a stride that holds them");

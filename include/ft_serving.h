@@ -85,7 +85,9 @@ int ft_rotary_run(const ft_rotary_handle* handle, const ft_rows* q, const ft_row
  * Strides are in elements, multiples of 16 bytes, the same for K and V; no two pages of
  * any layers share memory (layers may lie between pages); a page of a layer is dense in either order: (token_stride, head_stride) = (kv_heads * head_dim,
  * head_dim) or (head_dim, page_size * head_dim).  For the attention page_stride is a
- * multiple of 8 * token_stride, as it is for dense pages and for pages of K and V in turn. */
+ * multiple of 8 * token_stride, as it is for dense pages and for pages of K and V in turn.
+ * K and V must not share memory, except that one slab may be read as both (k == v) by the
+ * attention; appending to it and accepting in it are refused. */
 typedef struct {
   void* k;
   void* v;

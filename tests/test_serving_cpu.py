@@ -407,3 +407,13 @@ def test_layers_that_share_memory_are_refused(sv, ftg):
         assert (lib.ft_kv_cache_copy_pages(cache, None, None, 0, None) == ftg.FT_ERR_INVALID) == meet, (layer_stride, page_stride, layers, pages)
         seen[meet] += 1
     assert min(seen.values()) > 300
+
+
+def test_one_slab_as_k_and_v_cannot_be_written(sv, ftg):
+    lib, rows, x = sv._lib(), sv.FtRows(0x1000, 128, 64, 2), 0x1000
+    both = _cache(sv, v=0x10000)
+    assert lib.ft_kv_cache_append(both, 0, rows, rows, x, 1, None, None, None, None, None) == ftg.FT_ERR_INVALID
+    assert b"same memory" in lib.ft_gemm_last_error()
+    assert lib.ft_kv_cache_accept(both, x, 4, 4, x, x, x, x, 1, x + 64, None) == ftg.FT_ERR_INVALID
+    assert b"same memory" in lib.ft_gemm_last_error()
+    assert lib.ft_kv_cache_copy_pages(both, None, None, 0, None) == ftg.FT_OK
