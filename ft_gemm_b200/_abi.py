@@ -6,6 +6,7 @@ is no fallback path of any kind.
 """
 import ctypes
 import os
+import threading
 
 FT_OK = 0
 FT_ERR_INVALID = -1
@@ -50,13 +51,21 @@ class FtCacheView(ctypes.Structure):
 
 
 _lib = None
+_loading = threading.Lock()
 
 
 def load():
-    """Returns the loaded library; raises if it is missing (no fallback exists)."""
+    """Returns the loaded library; raises if it is missing (no fallback exists).  All threads get one object: the modules that
+    set more types on it do so once."""
     global _lib
-    if _lib is not None:
-        return _lib
+    if _lib is None:
+        with _loading:
+            if _lib is None:
+                _lib = _load()
+    return _lib
+
+
+def _load():
     if not os.path.exists(LIB_PATH):
         raise RuntimeError(
             f"{LIB_PATH} is missing: build it with `make lib` (or __graft_entry__.build()). "
@@ -97,7 +106,6 @@ def load():
                  "ft_gemm_fp8_abft_set_tolerance",
                  "ft_gemm_fp8_abft_host", "ft_gemm_generate_fp8", "ft_gemm_abi_version"):
         getattr(lib, name).restype = ci
-    _lib = lib
     return lib
 
 

@@ -7,6 +7,7 @@ memory and streams only; the reference has no counterpart to any of them.
 """
 import ctypes
 import struct
+import threading
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -57,49 +58,59 @@ _get_device, _raw_stream, _raw_alloc, _raw_delete = (
                                                "_cuda_cudaCachingAllocator_raw_delete"))
 
 _bound = False
+_binding = threading.Lock()
 _calls = {}  # the entry points that run on a device, with structures given as packed bytes
 
 
 def _lib():
-    global _bound
+    """The library with the types of this module's entry points.  The first use may come from several threads at once."""
+    global _bound, _calls
     lib = _abi.load()
     if not _bound:
-        vp, ci, rows, cache = ctypes.c_void_p, ctypes.c_int, ctypes.POINTER(FtRows), ctypes.POINTER(FtKvCache)
-        ints = ctypes.POINTER(ci)
-        lib.ft_rotary_options_default.argtypes = [ctypes.POINTER(FtRotaryOptions), ci]
-        lib.ft_rotary_options_default.restype = None
-        lib.ft_rotary_frequencies.argtypes = [ctypes.POINTER(FtRotaryOptions), ctypes.POINTER(ctypes.c_double)]
-        lib.ft_rotary_prepare.argtypes = [ctypes.POINTER(vp), ctypes.POINTER(FtRotaryOptions), vp]
-        lib.ft_rotary_destroy.argtypes = [vp]
-        lib.ft_rotary_run.argtypes = [vp, rows, rows, rows, rows, vp, ci, ci, ci, vp]
-        lib.ft_kv_cache_append.argtypes = [cache, ci, rows, rows, vp, ci, vp, vp, rows, rows, vp]
-        lib.ft_kv_cache_copy_pages.argtypes = [cache, vp, vp, ci, vp]
-        lib.ft_kv_cache_accept.argtypes = [cache, vp, ci, ci, vp, vp, vp, vp, ci, vp, vp]
-        lib.ft_page_pool_create.argtypes = [ctypes.POINTER(vp), ci, ci]
-        for name in ("destroy", "free_pages"):
-            getattr(lib, f"ft_page_pool_{name}").argtypes = [vp]
-        lib.ft_page_pool_new_sequence.argtypes = [vp, ints]
-        lib.ft_page_pool_fork.argtypes = [vp, ci, ints]
-        lib.ft_page_pool_free.argtypes = [vp, ci]
-        lib.ft_page_pool_extend.argtypes = [vp, ci, ci, ints, ints]
-        lib.ft_page_pool_truncate.argtypes = [vp, ci, ci]
-        lib.ft_page_pool_length.argtypes = [vp, ci]
-        lib.ft_page_pool_pages.argtypes = [vp, ci, ints, ci]
-        lib.ft_page_pool_compact.argtypes = [vp, ints, ints, ci, ints]
-        lib.ft_attention_workspace.argtypes = []
-        lib.ft_attention_workspace.restype = ctypes.c_size_t
-        lib.ft_prompt_attention_run.argtypes = [ctypes.POINTER(FtPromptAttentionArgs), vp, ctypes.c_size_t, vp, vp]
-        lib.ft_tree_attention_run.argtypes = [cache, ctypes.POINTER(FtTreeAttentionArgs), vp, ctypes.c_size_t, vp, vp]
-        lib.ft_tree_mask.argtypes = [ints, ci, ctypes.POINTER(ctypes.c_uint32), ci]
-        size = ctypes.c_size_t
-        for name, types in (("ft_rotary_run", [vp] * 6 + [ci] * 3 + [vp]), ("ft_kv_cache_append", [vp, ci, vp, vp, vp, ci] + [vp] * 5),
-                            ("ft_kv_cache_copy_pages", [vp, vp, vp, ci, vp]),
-                            ("ft_kv_cache_accept", [vp, vp, ci, ci, vp, vp, vp, vp, ci, vp, vp]),
-                            ("ft_prompt_attention_run", [vp, vp, size, vp, vp]), ("ft_tree_attention_run", [vp, vp, vp, size, vp, vp])):
-            _calls[name] = lib[name]
-            _calls[name].argtypes = types
-        _bound = True
+        with _binding:
+            if not _bound:
+                _calls = _bind(lib)
+                _bound = True
     return lib
+
+
+def _bind(lib) -> dict:
+    vp, ci, rows, cache = ctypes.c_void_p, ctypes.c_int, ctypes.POINTER(FtRows), ctypes.POINTER(FtKvCache)
+    ints = ctypes.POINTER(ci)
+    lib.ft_rotary_options_default.argtypes = [ctypes.POINTER(FtRotaryOptions), ci]
+    lib.ft_rotary_options_default.restype = None
+    lib.ft_rotary_frequencies.argtypes = [ctypes.POINTER(FtRotaryOptions), ctypes.POINTER(ctypes.c_double)]
+    lib.ft_rotary_prepare.argtypes = [ctypes.POINTER(vp), ctypes.POINTER(FtRotaryOptions), vp]
+    lib.ft_rotary_destroy.argtypes = [vp]
+    lib.ft_rotary_run.argtypes = [vp, rows, rows, rows, rows, vp, ci, ci, ci, vp]
+    lib.ft_kv_cache_append.argtypes = [cache, ci, rows, rows, vp, ci, vp, vp, rows, rows, vp]
+    lib.ft_kv_cache_copy_pages.argtypes = [cache, vp, vp, ci, vp]
+    lib.ft_kv_cache_accept.argtypes = [cache, vp, ci, ci, vp, vp, vp, vp, ci, vp, vp]
+    lib.ft_page_pool_create.argtypes = [ctypes.POINTER(vp), ci, ci]
+    for name in ("destroy", "free_pages"):
+        getattr(lib, f"ft_page_pool_{name}").argtypes = [vp]
+    lib.ft_page_pool_new_sequence.argtypes = [vp, ints]
+    lib.ft_page_pool_fork.argtypes = [vp, ci, ints]
+    lib.ft_page_pool_free.argtypes = [vp, ci]
+    lib.ft_page_pool_extend.argtypes = [vp, ci, ci, ints, ints]
+    lib.ft_page_pool_truncate.argtypes = [vp, ci, ci]
+    lib.ft_page_pool_length.argtypes = [vp, ci]
+    lib.ft_page_pool_pages.argtypes = [vp, ci, ints, ci]
+    lib.ft_page_pool_compact.argtypes = [vp, ints, ints, ci, ints]
+    lib.ft_attention_workspace.argtypes = []
+    lib.ft_attention_workspace.restype = ctypes.c_size_t
+    lib.ft_prompt_attention_run.argtypes = [ctypes.POINTER(FtPromptAttentionArgs), vp, ctypes.c_size_t, vp, vp]
+    lib.ft_tree_attention_run.argtypes = [cache, ctypes.POINTER(FtTreeAttentionArgs), vp, ctypes.c_size_t, vp, vp]
+    lib.ft_tree_mask.argtypes = [ints, ci, ctypes.POINTER(ctypes.c_uint32), ci]
+    size, calls = ctypes.c_size_t, {}
+    for name, types in (("ft_rotary_run", [vp] * 6 + [ci] * 3 + [vp]), ("ft_kv_cache_append", [vp, ci, vp, vp, vp, ci] + [vp] * 5),
+                        ("ft_kv_cache_copy_pages", [vp, vp, vp, ci, vp]),
+                        ("ft_kv_cache_accept", [vp, vp, ci, ci, vp, vp, vp, vp, ci, vp, vp]),
+                        ("ft_prompt_attention_run", [vp, vp, size, vp, vp]), ("ft_tree_attention_run", [vp, vp, vp, size, vp, vp])):
+        call = lib[name]
+        call.argtypes = types
+        calls[name] = call
+    return calls  # seen by others only now, when all have their types
 
 
 def _call(name: str, device: torch.device, *args):

@@ -6,6 +6,9 @@ import os
 import random
 import re
 import subprocess
+import threading
+import time
+import unittest.mock
 
 import pytest
 
@@ -417,3 +420,46 @@ def test_one_slab_as_k_and_v_cannot_be_written(sv, ftg):
     assert lib.ft_kv_cache_accept(both, x, 4, 4, x, x, x, x, 1, x + 64, None) == ftg.FT_ERR_INVALID
     assert b"same memory" in lib.ft_gemm_last_error()
     assert lib.ft_kv_cache_copy_pages(both, None, None, 0, None) == ftg.FT_OK
+
+
+def test_entry_points_are_seen_only_with_their_types(sv, monkeypatch):
+    """While one thread binds, another may call: an entry point without its types would cut addresses to 32 bits."""
+    real = sv._lib()
+
+    class Entry:
+        def __setattr__(self, name, value):
+            assert self not in sv._calls.values(), "published before its types were set"
+            object.__setattr__(self, name, value)
+
+    class Library:
+        def __getattr__(self, name):
+            return getattr(real, name)
+
+        def __getitem__(self, name):
+            return Entry()
+
+    library, names = Library(), set(sv._calls)
+    monkeypatch.setattr(sv._abi, "load", lambda: library)
+    monkeypatch.setattr(sv, "_bound", False)
+    monkeypatch.setattr(sv, "_calls", {})
+    assert sv._lib() is library
+    assert set(sv._calls) == names and all(hasattr(call, "argtypes") for call in sv._calls.values())
+
+
+def test_threads_that_load_at_once_get_one_library(sv, monkeypatch):
+    made = []
+
+    def slow(path):
+        time.sleep(0.05)
+        made.append(path)
+        return unittest.mock.MagicMock()
+
+    monkeypatch.setattr(sv._abi.ctypes, "CDLL", slow)
+    monkeypatch.setattr(sv._abi, "_lib", None)
+    got = []
+    threads = [threading.Thread(target=lambda: got.append(sv._abi.load())) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(made) == 1 and len(got) == 4 and all(x is got[0] for x in got)
