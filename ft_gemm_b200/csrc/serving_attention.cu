@@ -839,8 +839,9 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 const uint32_t* mask_row = p.mask + static_cast<long long>(item.token0 + (kSplitKeys ? 0 : x * tokens_per_half) + row_token) * p.mask_stride;
                 const int node = word0 - item.prefix;  // of the word's first key; negative before the first drafted token
                 const int word = node >> 5;
-                const uint32_t lo = word >= 0 && word < p.mask_words ? __ldg(mask_row + word) : 0u;
-                const uint32_t hi = word + 1 >= 0 && word + 1 < p.mask_words ? __ldg(mask_row + word + 1) : 0u;
+                // plain loads: the kernel in front, which may have written the mask, can still run when this one begins
+                const uint32_t lo = word >= 0 && word < p.mask_words ? mask_row[word] : 0u;
+                const uint32_t hi = word + 1 >= 0 && word + 1 < p.mask_words ? mask_row[word + 1] : 0u;
                 bits |= __funnelshift_r(lo, hi, node & 31);
                 const int there = min(max(item.keys - word0, 0), 32);
                 if (there < 32) bits &= (1u << there) - 1u;

@@ -787,6 +787,39 @@ def test_outputs_in_any_layout_whose_rows_are_apart(ftg, strides):
     assert torch.equal(out, want)
 
 
+def test_masks_written_just_in_front_of_the_call(ftg):
+    """The mask changes from call to call, written by the kernel in front on the same stream, in a graph as well."""
+    gen, dtype, page, n, m = _gen(42), torch.bfloat16, 32, 60, 200
+    cache = ftg.PagedCache.empty(1, 8, page, 2, 64, dtype)
+    cache.k.copy_(_randn(gen, cache.k.shape, dtype)), cache.v.copy_(_randn(gen, cache.v.shape, dtype))
+    q, out, op = _randn(gen, (n, 8, 64), dtype), torch.empty((n, 8, 64), dtype=dtype, device="cuda"), ftg.TreeAttention(8, cache)
+    args = 0, _offsets([n]), torch.arange(7, dtype=torch.int32, device="cuda")[None], torch.tensor([m], dtype=torch.int32, device="cuda")
+    masks = torch.randint(-2 ** 31, 2 ** 31, (6, n, 2), generator=gen, device="cuda").to(torch.int32)
+    want = []
+    for one in masks:
+        op.run(q, *args, out, mask=one)
+        torch.cuda.synchronize()
+        want.append(out.clone())
+    assert not any(torch.equal(a, b) for a, b in zip(want, want[1:]))
+    mask, got = torch.zeros_like(masks[0]), torch.empty((6, *out.shape), dtype=dtype, device="cuda")
+
+    def calls():
+        for i in range(6):
+            mask.copy_(masks[i])
+            op.run(q, *args, got[i], mask=mask)
+
+    calls()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls()
+    for replay in range(20):
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+        got.zero_(), mask.zero_()
+        graph.replay() if replay % 2 else calls()
+    op.report()
+
+
 def test_page_operations_and_rotary_positions_in_graphs_and_on_streams(ftg):
     gen, dtype = _gen(33), torch.bfloat16
     cache = ftg.PagedCache.empty(2, 12, 8, 2, 64, dtype)
