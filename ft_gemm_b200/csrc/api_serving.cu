@@ -665,7 +665,10 @@ static int attention_run(ServeAttentionParams& p, const ft_rows& q, const ft_row
   p.min_share = 1;
   // an upper bound on the units of work (serving_schedule.h), which are numbered in 31 bits
   const long long row_tiles = static_cast<long long>(p.query_tokens) / p.tokens_per_tile + p.batch;
-  if (row_tiles > INT32_MAX / 8 || row_tiles * p.kv_heads > INT32_MAX / (most_keys / 128 + 8)) {
+  const bool may_pass = row_tiles > INT32_MAX / 8 || row_tiles * p.kv_heads > INT32_MAX / (most_keys / 128 + 8);
+  // Several packed sequences have all keys between them, so the bound can be far off: the device counts.
+  p.count_units = may_pass && p.page_table == nullptr && p.batch > 1;
+  if (row_tiles > INT32_MAX / 8 || (may_pass && p.count_units == 0)) {
     return noalloc_fail(FT_ERR_INVALID, "the call is too large: %lld tiles of query rows for %d key heads over up to %lld keys", row_tiles, p.kv_heads, most_keys);
   }
   p.workspace = workspace;

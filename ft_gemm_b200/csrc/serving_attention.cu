@@ -373,8 +373,20 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   int first_sequence = 0;
   int left = 0, start = 0, share = 0, per_head = 1;  // units of the share; in front of it in its sequence; per CTA; per key head
   if (warp == 0) {
-    const int per_lane = (p.batch + 31) / 32;
-    const int scan_begin = min(lane * per_lane, p.batch), scan_end = min(scan_begin + per_lane, p.batch);
+    int batch = p.batch;
+    if (p.count_units != 0) {
+      long long most = 0;
+#pragma unroll 1
+      for (int i = lane; i < p.batch; i += 32) most += load_sequence(p, i, tokens_per_item, L::kItemCost).tiles.most_units_per_head() * p.kv_heads;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) most += __shfl_xor_sync(0xffffffffU, most, off);
+      if (most > 0x7fffffff) {  // nothing is done
+        batch = 0;
+        if (blockIdx.x == 0 && lane == 0) atomicExch(p.status, FT_ERR_INVALID);
+      }
+    }
+    const int per_lane = (batch + 31) / 32;
+    const int scan_begin = min(lane * per_lane, batch), scan_end = min(scan_begin + per_lane, batch);
     int mine = 0, before = 0, share_begin = 0, at = 0, found = scan_begin;
     bool holds = false;
     // first the sums; then the lane whose stretch holds the beginning goes through it once more, unless it is one sequence

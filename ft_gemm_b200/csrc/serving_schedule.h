@@ -19,8 +19,8 @@ namespace ftg {
 
 constexpr int kKeyTile = 128;
 
-// All units of a call are numbered in 31 bits (the caller refuses more: at a microsecond each they would take seconds on
-// every SM of the device).
+// All units of a call are numbered in 31 bits (more are refused: at a microsecond each they would take seconds on every SM
+// of the device).
 
 // sum over i in [0, n) of floor((a i + b) / 128) for a, b >= 0.  The steps repeat every 128 / gcd(a, 128) terms with an
 // increment of a / gcd(a, 128): one period is added up term by term (at most 128 of them; at most 4 for the usual head
@@ -87,6 +87,8 @@ struct SequenceTiles {
     if (r == row_tiles && row_tiles > 0) total += units_of(row_tiles - 1);
     return total;
   }
+  // at least the units of a key head, in 64 bits: every row tile with all keys
+  FT_HD long long most_units_per_head() const { return static_cast<long long>(row_tiles) * (tiles(keys) + item_cost); }
   FT_HD int units_per_head() const { return row_tiles == 0 ? 0 : units_before(row_tiles); }
 };
 

@@ -433,11 +433,14 @@ class _Attention:
             _abi.check(code)
 
     def report(self):
-        """Waits for the device and raises if a device-side wait of an earlier run gave up: its output is not valid."""
+        """Waits for the device and raises if the output of an earlier run is not valid: a device-side wait gave up, or packed
+        prompts made more tiles than can be numbered."""
         torch.cuda.synchronize(self.device)
         code = int(self.status.item())
         if code != _abi.FT_OK:
-            raise _abi.FtGemmError(code, "a device-side wait expired; the output of an earlier run is not valid")
+            why = "an earlier run had too many tiles and wrote nothing" if code == _abi.FT_ERR_INVALID else (
+                "a device-side wait expired; the output of an earlier run is not valid")
+            raise _abi.FtGemmError(code, why)
 
 
 class PromptAttention(_Attention):

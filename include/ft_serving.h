@@ -154,8 +154,10 @@ int ft_page_pool_compact(ft_page_pool* pool, int* host_sources, int* host_target
  * key gives zeros (and lse -inf).  head_dim is 64 or 128.  lse (may be NULL) is
  * float [token][head], the natural logarithm of the softmax denominator.  Output rows behind the
  * last sequence are left as they are.  `out` and lse overlap no input.  Packed k and v have at most
- * 2^27 rows, a page table holds at most 2^27 tokens, and calls of more than some 2^31 tiles of 128
- * rows by 128 keys are refused.
+ * 2^27 rows, and a page table holds at most 2^27 tokens.  A call has at most some 2^31 tiles of 128
+ * rows by 128 keys: counted with table_pages for each sequence over the cache, and with all of q and k
+ * for a single packed sequence, and refused beyond; several packed sequences are counted on the device,
+ * each with its own keys, and where they pass it the call writes FT_ERR_INVALID to `status` and no output.
  *
  * What lies behind a sequence's last key never reaches its output, whatever it is.  A key that some
  * rows of a sequence see and others do not has the probability zero in the others: K may hold
@@ -163,8 +165,8 @@ int ft_page_pool_compact(ft_page_pool* pool, int* host_sources, int* host_target
  *
  * `workspace` holds ft_attention_workspace() bytes, 16-byte aligned, contents arbitrary; calls that
  * can run at the same time need one each.  `status` is an int the caller sets to zero once; a
- * device-side wait that gives up writes FT_ERR_TIMEOUT there (the output is then not valid), and
- * nothing ever clears it. */
+ * device-side wait that gives up writes FT_ERR_TIMEOUT there (the output is then not valid), too many
+ * packed tiles FT_ERR_INVALID, and nothing ever clears it. */
 size_t ft_attention_workspace(void);
 
 /* Packed prompts: sequence b has the queries q_offsets[b] .. q_offsets[b+1] and the keys

@@ -820,6 +820,44 @@ def test_masks_written_just_in_front_of_the_call(ftg):
     op.report()
 
 
+def test_many_short_prompts_in_a_large_buffer(ftg):
+    """All tiles of rows times all keys pass 2^31, what the sequences really have is a small part of it: counted on the device."""
+    gen, dtype, batch, heads, d = _gen(43), torch.bfloat16, (1 << 17) + 5, 8, 64
+    rng = np.random.RandomState(43)
+    counts, key_counts = np.zeros(batch, dtype=np.int64), np.zeros(batch, dtype=np.int64)
+    some = sorted(rng.choice(batch, 40, replace=False))
+    counts[some], key_counts[some] = rng.randint(1, 200, 40), rng.randint(1, 500, 40)
+    tokens, keys = int(counts.sum()), 270_000
+    assert (tokens // 128 + batch) * heads * (keys // 128 + 8) > 2 ** 31
+    q, k, v = (_randn(gen, (n, heads, d), dtype) for n in (tokens + 3, keys, keys))
+    out = torch.full_like(q, 7.0)
+    op = ftg.PromptAttention(heads, heads, d, dtype=dtype)
+    offsets, key_offsets = _offsets(counts), _offsets(key_counts)
+    for _ in range(2):
+        op.run(q, k, v, out, offsets, key_offsets=key_offsets)
+    op.report()
+    a = b = 0
+    for n, m in zip(counts[some], key_counts[some]):
+        visible = torch.arange(m, device="cuda")[None] <= torch.arange(n, device="cuda")[:, None] + (int(m) - int(n))
+        _check_rows(out[a:a + n], None, q[a:a + n], k[b:b + m], v[b:b + m], visible, d ** -0.5)
+        a, b = a + n, b + m
+    assert bool((out[tokens:] == 7.0).all())
+
+
+def test_packed_prompts_of_too_many_tiles_say_so_and_write_nothing(ftg):
+    dtype, heads, n, m = torch.bfloat16, 128, 34_000, 1 << 24
+    assert (n // 2) * (m // 128) > 2 ** 31  # 2 tiles of one token's heads at a time
+    q, k = torch.zeros((n + 1, heads, 64), dtype=dtype, device="cuda"), torch.zeros((m + 1, 1, 64), dtype=dtype, device="cuda")
+    out = torch.full_like(q, 7.0)
+    op = ftg.PromptAttention(heads, 1, 64, dtype=dtype)
+    op.run(q, k, k, out, _offsets([n, 1]), key_offsets=_offsets([m, 1]))
+    with pytest.raises(ftg.FtGemmError, match="too many tiles"):
+        op.report()
+    assert bool((out == 7.0).all())
+    with pytest.raises(ftg.FtGemmError, match="too large"):  # one sequence: known before the launch
+        op.run(q, k, k, out, _offsets([n]), key_offsets=_offsets([m]))
+
+
 def test_page_operations_and_rotary_positions_in_graphs_and_on_streams(ftg):
     gen, dtype = _gen(33), torch.bfloat16
     cache = ftg.PagedCache.empty(2, 12, 8, 2, 64, dtype)
