@@ -267,6 +267,8 @@ class PagedCache:
         if rotary is not None:
             if rotary.device != device or rotary.head_dim != head_dim:
                 raise ValueError(f"the rotary positions must be on {device} for heads of {head_dim}")
+            if not rotary.handle.value:
+                raise ValueError("the rotary positions are closed")  # to the library that would be an append without them
             handle, at = rotary.handle, _vector(positions, "positions", torch.int64, device, tokens)
         if q is not None:
             if q.dim() != 3:

@@ -8,6 +8,7 @@ import re
 import subprocess
 import threading
 import time
+import types
 import unittest.mock
 
 import pytest
@@ -463,3 +464,15 @@ def test_threads_that_load_at_once_get_one_library(sv, monkeypatch):
     for t in threads:
         t.join()
     assert len(made) == 1 and len(got) == 4 and all(x is got[0] for x in got)
+
+
+def test_appending_with_closed_rotary_positions_is_refused(sv, ftg):
+    """Not K as it is, as if no positions had been given."""
+    torch = pytest.importorskip("torch")
+    here = types.SimpleNamespace(index=-1)  # where tensors on the host say they are
+    cache, rotary = object.__new__(ftg.PagedCache), object.__new__(ftg.Rotary)
+    cache.device, cache.dtype, cache.kv_heads, cache.head_dim, cache.address = here, torch.bfloat16, 2, 64, 0
+    rotary.device, rotary.head_dim, rotary.handle = here, 64, ctypes.c_void_p()
+    k, at = torch.zeros((3, 2, 64), dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="closed"):
+        cache.append(0, k, k, at, rotary=rotary, positions=at)
