@@ -25,6 +25,8 @@ namespace {
     if (err_ != cudaSuccess) return noalloc_fail(FT_ERR_CUDA, "%s failed: %s", #call, cudaGetErrorString(err_)); \
   } while (0)
 
+constexpr float kLog2E = 1.44269504088896340736f;
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // The rules every ft_rows has to meet; `heads` is what the operator expects there.
@@ -117,7 +119,9 @@ int check_two_slabs(const ft_kv_cache* c) {
 }
 
 int check_scale(float scale) {
-  if (!(scale >= 0.0f) || !std::isfinite(scale)) return noalloc_fail(FT_ERR_INVALID, "scale must be positive and finite (0: 1 / sqrt(head_dim))");
+  if (!(scale >= 0.0f) || !std::isfinite(kLog2E * scale)) {  // the exponents are in units of log2(e) * scale
+    return noalloc_fail(FT_ERR_INVALID, "scale must be positive and below 2.3e38 (0: 1 / sqrt(head_dim))");
+  }
   return FT_OK;
 }
 
@@ -237,8 +241,8 @@ int ft_rotary_frequencies(const ft_rotary_options* o, double* out) {
     return noalloc_fail(FT_ERR_INVALID, "head_dim (at most 256) and rotary_dim (at most head_dim) must be positive multiples of 16 (got %d, %d)",
                         o->head_dim, o->rotary_dim);
   }
-  if (!(o->base > 0.0) || !std::isfinite(o->base) || !(o->factor > 0.0) || !std::isfinite(o->factor) || !std::isfinite(o->magnitude)) {
-    return noalloc_fail(FT_ERR_INVALID, "base and factor must be positive, magnitude finite");
+  if (!(o->base > 0.0) || !std::isfinite(o->base) || !(o->factor > 0.0) || !std::isfinite(o->factor) || !std::isfinite(static_cast<float>(o->magnitude))) {
+    return noalloc_fail(FT_ERR_INVALID, "base and factor must be positive, magnitude finite in 32 bits");
   }
   if (o->scaling < FT_ROTARY_PLAIN || o->scaling > FT_ROTARY_BY_PARTS) return noalloc_fail(FT_ERR_INVALID, "unknown scaling %d", o->scaling);
   if (o->scaling == FT_ROTARY_BY_PARTS &&
@@ -255,6 +259,7 @@ int ft_rotary_frequencies(const ft_rotary_options* o, double* out) {
       const double keep = std::min(1.0, std::max(0.0, (o->original_length * f / two_pi - o->low) / (o->high - o->low)));
       f *= keep + (1.0 - keep) / o->factor;
     }
+    if (!std::isfinite(f) || !std::isfinite(base)) return noalloc_fail(FT_ERR_INVALID, "base and factor give frequencies that are not finite");
     out[i] = f;
   }
   return FT_OK;
@@ -661,7 +666,7 @@ static int attention_run(ServeAttentionParams& p, const ft_rows& q, const ft_row
   p.heads = q.heads;
   p.group = q.heads / p.kv_heads;
   p.tokens_per_tile = 128 / p.group;
-  p.scale_log2 = 1.44269504088896340736f * (scale != 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(p.head_dim)));
+  p.scale_log2 = kLog2E * (scale != 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(p.head_dim)));
   p.min_share = 1;
   // an upper bound on the units of work (serving_schedule.h), which are numbered in 31 bits
   const long long row_tiles = static_cast<long long>(p.query_tokens) / p.tokens_per_tile + p.batch;

@@ -476,3 +476,14 @@ def test_appending_with_closed_rotary_positions_is_refused(sv, ftg):
     k, at = torch.zeros((3, 2, 64), dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int64)
     with pytest.raises(ValueError, match="closed"):
         cache.append(0, k, k, at, rotary=rotary, positions=at)
+
+
+def test_numbers_that_leave_their_range_are_refused(sv, ftg):
+    """A scale times log2(e), a magnitude in 32 bits, frequencies and a grown base that would be infinite."""
+    for bad in (dict(magnitude=1e39), dict(magnitude=-1e39), dict(scaling=1, factor=1e-310), dict(scaling=2, base=1e300, factor=1e300)):
+        assert _frequencies(sv, **bad)[0] == ftg.FT_ERR_INVALID, bad
+    assert _frequencies(sv, magnitude=3e38)[0] == ftg.FT_OK and _frequencies(sv, scaling=2, base=1e150, factor=1e150)[0] == ftg.FT_OK
+    rows = lambda heads: sv.FtRows(0x10000, heads * 128, 128, heads)  # noqa: E731
+    for scale, batch, code in ((3e38, 1, ftg.FT_ERR_INVALID), (2.36e38, 1, ftg.FT_ERR_INVALID), (2.3e38, 0, ftg.FT_OK)):
+        a = sv.FtPromptAttentionArgs(rows(8), rows(2), rows(2), rows(8), None, 0x1000, None, batch, 16, 16, 128, 1, 1, scale)
+        assert sv._lib().ft_prompt_attention_run(a, 0x100000, 1 << 40, 0x1000, None) == code
