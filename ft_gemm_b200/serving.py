@@ -350,6 +350,10 @@ class PagePool:
         out = (ctypes.c_int * self.pages)()
         return list(out[:self._value(self.lib.ft_page_pool_pages(self.handle, sequence, out, self.pages))])
 
+    def _check_stream(self, stream: Optional[torch.cuda.Stream]):
+        if stream is not None and self.cache is not None:
+            _stream(self.cache.device, stream)  # refuses another device's, before anything changes
+
     def _move(self, pairs: List[Tuple[int, int]], stream: Optional[torch.cuda.Stream]):
         if pairs and self.cache is not None:
             with torch.cuda.stream(stream) if stream is not None else torch.cuda.device(self.cache.device):
@@ -362,6 +366,7 @@ class PagePool:
         their room."""
         if len(sequences) != len(counts):
             raise ValueError("one count for each sequence")
+        self._check_stream(stream)
         pairs = []
         try:
             for sequence, count in zip(sequences, counts):
@@ -375,6 +380,7 @@ class PagePool:
 
     def compact(self, stream: Optional[torch.cuda.Stream] = None) -> List[Tuple[int, int]]:
         """Moves the used pages to the front of the cache; page tables made before are no longer right."""
+        self._check_stream(stream)
         a, b, n = (ctypes.c_int * self.pages)(), (ctypes.c_int * self.pages)(), ctypes.c_int()
         _abi.check(self.lib.ft_page_pool_compact(self.handle, a, b, self.pages, ctypes.byref(n)))
         pairs = list(zip(a[:n.value], b[:n.value]))

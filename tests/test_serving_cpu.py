@@ -487,3 +487,19 @@ def test_numbers_that_leave_their_range_are_refused(sv, ftg):
     for scale, batch, code in ((3e38, 1, ftg.FT_ERR_INVALID), (2.36e38, 1, ftg.FT_ERR_INVALID), (2.3e38, 0, ftg.FT_OK)):
         a = sv.FtPromptAttentionArgs(rows(8), rows(2), rows(2), rows(8), None, 0x1000, None, batch, 16, 16, 128, 1, 1, scale)
         assert sv._lib().ft_prompt_attention_run(a, 0x100000, 1 << 40, 0x1000, None) == code
+
+
+def test_the_pool_refuses_streams_of_another_device(ftg):
+    """Its copies would run on another stream than the caller orders them by; nothing has changed then."""
+    torch = pytest.importorskip("torch")
+    pool = ftg.PagePool(6, 4)
+    free, a = pool.new_sequence(), pool.new_sequence()
+    pool.extend([free, a], [3, 6])
+    pool.fork(a)
+    pool.free(free)  # a hole in front of the used pages, and a last page that two sequences hold
+    pool.cache = types.SimpleNamespace(pages=6, page_size=4, device=torch.device("cuda:0"))
+    before, other = pool.page_list(a), types.SimpleNamespace(device=torch.device("cuda:1"), cuda_stream=0)
+    for call in (lambda: pool.extend([a], [1], stream=other), lambda: pool.compact(stream=other)):
+        with pytest.raises(ValueError, match="stream belongs to"):
+            call()
+        assert pool.page_list(a) == before and pool.length(a) == 6 and pool.free_pages() == 4
