@@ -896,10 +896,11 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             }
           }
           // The probabilities are rounded to 16 bits once, as an operand of the second product; the denominator adds up the numbers
-          // before that, so that a row's roundings, of either sign, do not weigh on all of its values together.
+          // before that, so that a row's roundings, of either sign, do not weigh on all of its values together.  A tile's 64 are added up
+          // by themselves: one at a time, small numbers would be lost beside the sum of many keys.
           const float base = reference == -INFINITY ? 0.0f : reference;
           const unsigned long long scale2 = pack_f32x2(p.scale_log2, p.scale_log2), base2 = pack_f32x2(-base, -base);
-          unsigned long long sum_a = pack_f32x2(sum, 0.0f), sum_b = pack_f32x2(0.0f, 0.0f);
+          unsigned long long sum_a = pack_f32x2(0.0f, 0.0f), sum_b = pack_f32x2(0.0f, 0.0f);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t packed[16];
@@ -925,7 +926,7 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           }
           float lo, hi;
           unpack_f32x2(add_f32x2(sum_a, sum_b), lo, hi);
-          sum = lo + hi;
+          sum += lo + hi;
           tmem_wait_st();
         }
         tcgen05_fence_before();

@@ -858,6 +858,30 @@ def test_packed_prompts_of_too_many_tiles_say_so_and_write_nothing(ftg):
         op.run(q, k, k, out, _offsets([n]), key_offsets=_offsets([m]))
 
 
+def _same_page_over_and_over(ftg, dim, keys, queries):
+    """A chain of `queries` zeros over `keys` tokens that all lie in one page, V all ones: (out, lse, how many keys each row sees)."""
+    dtype, page = torch.bfloat16, 256
+    cache = ftg.PagedCache.empty(1, 1, page, 1, dim, dtype)
+    cache.k.fill_(0.5), cache.v.fill_(1.0)
+    q = torch.zeros((queries, 1, dim), dtype=dtype, device="cuda")
+    out, lse = torch.full_like(q, 7.0), torch.empty((queries, 1), device="cuda")
+    table = torch.zeros((1, -(-keys // page)), dtype=torch.int32, device="cuda")
+    op = ftg.TreeAttention(1, cache)
+    op.run(q, 0, _offsets([queries]), table, torch.tensor([keys], dtype=torch.int32, device="cuda"), out, lse=lse)
+    op.report()
+    return out, lse, torch.arange(keys - queries + 1, keys + 1, device="cuda")
+
+
+def test_the_sum_of_very_many_equal_probabilities(ftg):
+    """2^26 keys of probability one for every CTA: counts of 64 and their multiples, exact in 32 bits, but ones added to a sum of 2^24
+    and more are lost one by one.  The logarithm: a few roundings of a number of its size."""
+    rows = 256 * torch.cuda.get_device_properties(0).multi_processor_count
+    out, lse, seen = _same_page_over_and_over(ftg, 64, 1 << 26, rows)
+    assert bool((out == 1.0).all()), out.float().max().item()
+    want = seen.double().log()[:, None]
+    assert bool(((lse.double() - want).abs() <= 2.0 ** -21 * (1 + want)).all())
+
+
 def test_page_operations_and_rotary_positions_in_graphs_and_on_streams(ftg):
     gen, dtype = _gen(33), torch.bfloat16
     cache = ftg.PagedCache.empty(2, 12, 8, 2, 64, dtype)
