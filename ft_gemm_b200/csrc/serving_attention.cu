@@ -37,11 +37,15 @@ namespace {
 
 constexpr int kRows = 128;     // rows of a tile: the lanes of tensor memory
 constexpr int kRoleWarps = 3;  // in front of the softmax warps
-// 96 registers each.  Nothing spills in the loops: spills go to an L1 cache that shared memory has left little of.
+// 96 registers each.  Nothing spills: spills would go to an L1 cache that shared memory has left little of.
 constexpr int kThreads = (kRoleWarps + 16) * 32;
 constexpr uint32_t kTimeoutNs = 2000000000u;
 constexpr float kRescaleStep = 8.0f;  // log2 units
 constexpr int kItems = 4;             // descriptors in flight
+// The tensor core cuts each product off some 2^-25 below the sum it is added to, always towards zero: over N keys that is up to
+// N 2^-27 of the sum (equal values, one row tile per CTA: 0.5 % too small after 2^20 keys, 11 % after 2^24).  After so many of its
+// key tiles a side adds its accumulator to a copy in the workspace and begins anew, so no more than 2^17 keys, 2^-10, weigh on a sum.
+constexpr int kKeepTiles = 1024;
 constexpr int kMaxStages = 12;
 constexpr uint32_t kTmemS = 0, kTmemO = 256;  // S of A and B: 128 columns each; O of A and B: kDim each
 
@@ -68,6 +72,7 @@ struct Shared {
   uint64_t state_full[2];    // [side] (kSplitKeys: the first for both)
   float row_max[2][2][kRows];     // [side][key half]; written again only when the next scores are there, which follows both reads
   float2 state[2][2][2][kRows];   // [item parity][side][key half]: {reference, sum} of the rows, in turn for odd and even items
+  float2 kept[2][2][kRows];       // [side][key half]: {reference, sum} of what the sides have put into the workspace
 };
 
 template <int kDim, bool kSplitKeys>
@@ -281,6 +286,58 @@ __device__ __forceinline__ Item load_item(const volatile Item& from) {
   i.end = from.end;
   i.slot = from.slot;
   return i;
+}
+
+// Where a warpgroup keeps its half of the columns of its side's accumulator, [column / 4][row]: the place of the item's own part, or,
+// for a whole row tile, of the part that only the CTA's last item can have.
+template <int kDim>
+__device__ __forceinline__ float4* kept_at(void* workspace, int slot, int side, int column_half) {
+  return parts_of(workspace, gridDim.x).o + (((static_cast<size_t>(blockIdx.x) * 2 + (slot < 0 ? 1 : slot)) * 2 + side) * (kDim / 4) + column_half * (kDim / 8)) * kRows;
+}
+// Adds this thread's columns of the accumulator and its sum to what is kept (`again`: something is) and begins anew; or, `back`,
+// adds what is kept to the accumulator and to the sum that it returns.
+template <int kDim>
+__device__ __forceinline__ float keep_accumulator(uint32_t o_addr, float4* o_kept, float2* kept, float reference, float sum, bool again, bool back) {
+  tcgen05_fence_after();
+  float shrink = 0.0f;
+  if (again) {
+    shrink = exp2_approx(kept->x - (reference == -INFINITY ? 0.0f : reference));
+    sum = fmaf(kept->y, shrink, sum);
+  }
+#pragma unroll 1
+  for (int d = 0; d < kDim / 2; d += 8, o_kept += 2 * kRows) {
+    float o[8];
+    tmem_ld_32x32b_x8(o_addr + d, o);
+    tmem_wait_ld();
+    if (again) {
+      const float4 a = o_kept[0], b = o_kept[kRows];
+      o[0] = fmaf(a.x, shrink, o[0]);
+      o[1] = fmaf(a.y, shrink, o[1]);
+      o[2] = fmaf(a.z, shrink, o[2]);
+      o[3] = fmaf(a.w, shrink, o[3]);
+      o[4] = fmaf(b.x, shrink, o[4]);
+      o[5] = fmaf(b.y, shrink, o[5]);
+      o[6] = fmaf(b.z, shrink, o[6]);
+      o[7] = fmaf(b.w, shrink, o[7]);
+    }
+    if (!back) {
+      o_kept[0] = make_float4(o[0], o[1], o[2], o[3]);
+      o_kept[kRows] = make_float4(o[4], o[5], o[6], o[7]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = 0.0f;
+    }
+    tmem_st_32x32b_x8(o_addr + d, o);
+  }
+  tmem_wait_st();
+  tcgen05_fence_before();
+  if (back) return sum;
+  *kept = make_float2(reference, sum);
+  return 0.0f;
+}
+
+template <int kDim>
+__device__ __noinline__ float keep_accumulator_call(uint32_t o_addr, float4* o_kept, float2* kept, float reference, float sum, bool again) {
+  return keep_accumulator<kDim>(o_addr, o_kept, kept, reference, sum, again, false);
 }
 
 // In pairs the unit for exponentials has as much to do as the tensor core (a tile's 128 x 128 take it 1024 cycles, the two
@@ -836,6 +893,14 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         if (!ok) break;
         s_phase ^= 1;
         tcgen05_fence_after();
+        // the accumulator is complete up to the tile before this one, and this one's products wait for both warpgroups
+        if ((i & (kKeepTiles - 1)) == 0 && i > 0 && warp_has_rows) {
+          // In line or called, whichever leaves the loop its registers: long trees with heads of 64 164 us and 153, 4 x 4096 packed tokens 499
+          // and 535 us; without this branch 153 and 495.
+          float4* to = kept_at<kDim>(p.workspace, item.slot, x, c) + row;
+          sum = kPaged ? keep_accumulator_call<kDim>(o_addr, to, &sh.kept[x][c][row], reference, sum, i > kKeepTiles)
+                       : keep_accumulator<kDim>(o_addr, to, &sh.kept[x][c][row], reference, sum, i > kKeepTiles, false);
+        }
         if (warp_has_rows) {
           float s[64];
           tmem_ld_32x32b_x32(s_addr, s);
@@ -945,6 +1010,9 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       if (count_a > 0) o_phase ^= 1;
       if (count_b > 0) o_phase ^= 2;
       const int parity = index & 1;
+      if (count > kKeepTiles && warp_has_rows) {
+        sum = keep_accumulator<kDim>(o_addr, kept_at<kDim>(p.workspace, item.slot, x, c) + row, &sh.kept[x][c][row], reference, sum, true, true);
+      }
       sh.state[parity][x][c][row] = make_float2(reference, sum);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.state_full[kSplitKeys ? 0 : x]);

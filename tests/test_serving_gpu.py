@@ -882,6 +882,105 @@ def test_the_sum_of_very_many_equal_probabilities(ftg):
     assert bool(((lse.double() - want).abs() <= 2.0 ** -21 * (1 + want)).all())
 
 
+def _repeated_pages(ftg, gen, dim, dtype, lengths, queries, pages, order, heads=2, climb=0.0):
+    """Chains over caches whose page table names a few pages of 256 tokens many times: sequence b has the pages order(b), repeated
+    as they stand, up to lengths[b].  Checks out and lse in 64 bits by counting how often each row sees each token of a page."""
+    page = 256
+    cache = ftg.PagedCache.empty(1, pages, page, 1, dim, dtype)
+    side = torch.randint(0, 2, (dim,), generator=gen, device="cuda") * 2.0 - 1.0
+    q = (side * (torch.rand((sum(queries), heads, 1), generator=gen, device="cuda") + 0.2) * (64 / dim) ** 0.5).to(dtype)
+    step = torch.arange(pages, device="cuda")[:, None, None, None] * climb
+    cache.k[0].copy_(side * step + torch.randn(cache.k[0].shape, generator=gen, device="cuda"))
+    cache.v.copy_(torch.rand(cache.v.shape, generator=gen, device="cuda") + 0.5)  # no two signs: nothing cancels
+    width = -(-max(lengths) // page)
+    table = torch.stack([order(b, width) for b in range(len(lengths))]).to(torch.int32)
+    out, lse, op = torch.full_like(q, 7.0), torch.empty((len(q), heads), device="cuda"), ftg.TreeAttention(heads, cache)
+    op.run(q, 0, _offsets(queries), table.cuda(), torch.tensor(lengths, dtype=torch.int32, device="cuda"), out, lse=lse)
+    op.report()
+    kd, vd = cache.k[0].double().reshape(-1, dim), cache.v[0].double().reshape(-1, dim)
+    u, at = _half_eps(dtype), 0
+    for b, (m, n) in enumerate(zip(lengths, queries)):
+        seen = torch.arange(m - n + 1, m + 1)  # per row
+        whole, rest = seen // page, seen % page
+        times = torch.zeros((n, pages), dtype=torch.int64)
+        first = int(whole[0])
+        times += torch.bincount(table[b, :first].long(), minlength=pages)
+        for j in range(first, int(whole[-1])):  # pages that only the later rows see in full
+            times[:, int(table[b, j])] += (whole > j).long()
+        count = times[:, :, None].expand(n, pages, page).clone()
+        last = table[b].long()[whole.clamp(max=width - 1)]
+        count[torch.arange(n), last] += (torch.arange(page)[None] < rest[:, None]).long()
+        count = count.reshape(n, -1).cuda().double()
+        for h in range(heads):
+            rows = slice(at, at + n)
+            x = (q[rows, h].double() @ kd.T) * dim ** -0.5
+            size = ((q[rows, h].double().abs() @ kd.abs().T) * dim ** -0.5).max().item()
+            top = x.masked_fill(count == 0, -math.inf).amax(-1, keepdim=True)
+            e = count * torch.exp(x - top)
+            total = e.sum(-1, keepdim=True)
+            want = e @ vd / total  # also the weighted mean of |v|
+            s = (dim + 8) * 2.0 ** -24 * max(size, 1.0)
+            bound = 1.02 * (2 * u + 2 * s + 2.0 ** -10 + 2.0 ** -13) * want + max(lengths) * 2.0 ** -32 * 1.5
+            off = (out[rows, h].double() - want).abs()
+            assert bool((off <= bound).all()), f"sequence {b}: off by {(off / want).max().item()}, {(off / bound).max().item()} of the bound"
+            want = (top + torch.log(total))[:, 0]
+            assert bool(((lse[rows, h].double() - want).abs() <= s + 2.0 ** -13 + 2.0 ** -21 * (1 + want.abs())).all())
+        at += n
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", ["pairs", "split"])
+@pytest.mark.parametrize("climb", [0.0, 0.6])
+def test_millions_of_keys(ftg, dim, dtype, rows, climb):
+    """More key tiles of one row tile on one CTA than a side adds up at once (1024, 2^17 keys: at most N 2^-27 = 2^-10 of the sum is cut off;
+    2 x 1024 further additions, 2^-13); page after page of larger scores when they climb, so that what is kept shrinks."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    pages = 8
+    in_turn = lambda b, width: torch.arange(width) * pages // width if climb else (torch.arange(width) + b) % pages  # noqa: E731
+    if rows == "pairs":
+        _repeated_pages(ftg, _gen(45), dim, DTYPES[dtype], [600_001, 2_000_123], [64 * sms + 77, 64 * sms], pages, in_turn, climb=climb)
+    else:
+        lengths = [1_000_001 + 9973 * b for b in range(60)]
+        _repeated_pages(ftg, _gen(46), dim, DTYPES[dtype], lengths, [1] * 60, pages, in_turn, climb=climb)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", ["pairs", "split"])
+def test_millions_of_packed_keys(ftg, dim, dtype, rows):
+    """The same over packed keys, growing towards the end; some of the rows are checked."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    gen, dtype, heads = _gen(47), DTYPES[dtype], 2
+    n, m = (128 * sms, 300_001) if rows == "pairs" else (1, 2 * 1200 * 128 * sms + 77)
+    side = torch.randint(0, 2, (dim,), generator=gen, device="cuda") * 2.0 - 1.0
+    q = (side * (torch.rand((n, heads, 1), generator=gen, device="cuda") + 0.2) * (64 / dim) ** 0.5).to(dtype)
+    k, v = torch.empty((m, 1, dim), dtype=dtype, device="cuda"), torch.empty((m, 1, dim), dtype=dtype, device="cuda")
+    pieces = [(a, min(a + (1 << 20), m)) for a in range(0, m, 1 << 20)]
+    for a, b in pieces:
+        grow = torch.arange(a, b, device="cuda")[:, None, None] * (4.0 / m)
+        k[a:b] = side * grow + torch.randn((b - a, 1, dim), generator=gen, device="cuda")
+        v[a:b] = torch.rand((b - a, 1, dim), generator=gen, device="cuda") + 0.5
+    out, lse, op = torch.full_like(q, 7.0), torch.empty((n, heads), device="cuda"), ftg.PromptAttention(heads, 1, dim, dtype=dtype)
+    op.run(q, k, v, out, _offsets([n]), key_offsets=_offsets([m]), lse=lse)
+    op.report()
+    some = torch.tensor(sorted({0, n // 3, n // 2, n - 1}), device="cuda")
+    x = [(q[some].double().reshape(-1, dim) @ k[a:b, 0].double().T) * dim ** -0.5 for a, b in pieces]
+    sees = (some + m - n).repeat_interleave(heads)[:, None]  # the last key of each row
+    x = torch.cat(x, 1).masked_fill(torch.arange(m, device="cuda")[None] > sees, -math.inf)
+    size = x.masked_fill(x == -math.inf, 0.0).abs().max().item() + 8.0 * dim ** 0.5  # of the sum of magnitudes: |q| |k| is at most some units more
+    top = x.amax(-1, keepdim=True)
+    e = torch.exp(x - top)
+    total = e.sum(-1, keepdim=True)
+    want = sum(e[:, a:b] @ v[a:b, 0].double() for a, b in pieces) / total
+    u, s = _half_eps(dtype), (dim + 8) * 2.0 ** -24 * size
+    bound = 1.02 * (2 * u + 2 * s + 2.0 ** -10 + 2.0 ** -13) * want + m * 2.0 ** -32 * 1.5
+    off = (out[some].double().reshape(-1, dim) - want).abs()
+    assert bool((off <= bound).all()), f"off by {(off / want).max().item()}, {(off / bound).max().item()} of the bound"
+    want = (top + torch.log(total))[:, 0]
+    assert bool(((lse[some].double().reshape(-1) - want).abs() <= s + 2.0 ** -13 + 2.0 ** -21 * (1 + want.abs())).all())
+
+
 def test_page_operations_and_rotary_positions_in_graphs_and_on_streams(ftg):
     gen, dtype = _gen(33), torch.bfloat16
     cache = ftg.PagedCache.empty(2, 12, 8, 2, 64, dtype)
