@@ -633,8 +633,8 @@ size_t ft_attention_workspace(void) {
 }
 
 constexpr int kMaxQueries = 1 << 30;  // sums of a few of them stay inside 32 bits
-// A warp that has nothing to do for a row tile waits while the others go through its keys, and waits give up after 2
-// seconds: 2^20 key tiles take about one.
+// A warp that has nothing to do for a row tile waits while the others go through its keys, and waits give up after 4
+// seconds: 2^20 key tiles take 2 to 3.
 constexpr int kMaxKeys = 1 << 27;
 
 static int check_heads(int heads, int kv_heads) {

@@ -39,7 +39,10 @@ constexpr int kRows = 128;     // rows of a tile: the lanes of tensor memory
 constexpr int kRoleWarps = 3;  // in front of the softmax warps
 // 96 registers each.  Nothing spills: spills would go to an L1 cache that shared memory has left little of.
 constexpr int kThreads = (kRoleWarps + 16) * 32;
-constexpr uint32_t kTimeoutNs = 2000000000u;
+// A role that has nothing to do for an item waits while the others go through its keys: up to 2^20 tiles of them (2^27 keys), at
+// 2.1 us for two tiles of rows with heads of 128 and 1.9 GHz, 3.1 where the power cap holds the clock at 1.3 GHz.  (The timer's
+// low word counts to 4.29 s.)
+constexpr uint32_t kTimeoutNs = 4000000000u;
 constexpr float kRescaleStep = 8.0f;  // log2 units
 constexpr int kItems = 4;             // descriptors in flight
 // The tensor core cuts each product off some 2^-25 below the sum it is added to, always towards zero: over N keys that is up to

@@ -981,6 +981,16 @@ def test_millions_of_packed_keys(ftg, dim, dtype, rows):
     assert bool(((lse[some].double().reshape(-1) - want).abs() <= s + 2.0 ** -13 + 2.0 ** -21 * (1 + want.abs())).all())
 
 
+def test_a_row_tile_over_as_many_keys_as_there_can_be(ftg):
+    """2^27 keys in one item per CTA (seconds of work): the warp that clears the rows behind the last key waits for all of it.  The sums:
+    multiples of 64 up to 2^26 for each half of the keys, then one addition."""
+    keys, rows = (1 << 27) - 5, 256 * torch.cuda.get_device_properties(0).multi_processor_count
+    out, lse, seen = _same_page_over_and_over(ftg, 128, keys, rows)
+    assert bool((out == 1.0).all()), (out.float().min().item(), out.float().max().item())
+    want = seen.double().log()[:, None]
+    assert bool(((lse.double() - want).abs() <= 2.0 ** -21 * (1 + want)).all())
+
+
 def test_page_operations_and_rotary_positions_in_graphs_and_on_streams(ftg):
     gen, dtype = _gen(33), torch.bfloat16
     cache = ftg.PagedCache.empty(2, 12, 8, 2, 64, dtype)
