@@ -667,7 +667,6 @@ static int attention_run(ServeAttentionParams& p, const ft_rows& q, const ft_row
   p.group = q.heads / p.kv_heads;
   p.tokens_per_tile = 128 / p.group;
   p.scale_log2 = kLog2E * (scale != 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(p.head_dim)));
-  p.min_share = 1;
   // an upper bound on the units of work (serving_schedule.h), which are numbered in 31 bits
   const long long row_tiles = static_cast<long long>(p.query_tokens) / p.tokens_per_tile + p.batch;
   const bool may_pass = row_tiles > INT32_MAX / 8 || row_tiles * p.kv_heads > INT32_MAX / (most_keys / 128 + 8);

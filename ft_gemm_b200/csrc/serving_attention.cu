@@ -474,7 +474,7 @@ serve_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       }
       const int total = __shfl_sync(0xffffffffU, before, 31);
       before -= mine;
-      share = max(total / static_cast<int>(gridDim.x) + 1, p.min_share);
+      share = total / static_cast<int>(gridDim.x) + 1;
       share_begin = static_cast<int>(min(static_cast<long long>(share) * blockIdx.x, static_cast<long long>(total)));
       left = min(share, total - share_begin);
       holds = left > 0 && before <= share_begin && share_begin < before + mine;

@@ -64,7 +64,6 @@ struct ServeAttentionParams {
   int tokens_per_tile;  // 128 / group: tokens whose heads fill a tile of 128 rows
   int page_size, pages, table_pages, table_stride;
   int page_groups;   // groups of 8 tokens from page to page
-  int min_share;     // key tiles that a CTA takes at least
   int count_units;   // the host could not tell that the units of work stay inside 31 bits
   float scale_log2;  // log2(e) * scale
   void* workspace;
