@@ -991,6 +991,60 @@ def test_a_row_tile_over_as_many_keys_as_there_can_be(ftg):
     assert bool(((lse.double() - want).abs() <= 2.0 ** -21 * (1 + want)).all())
 
 
+def test_a_call_waits_for_what_another_stream_has_written(ftg):
+    """Its kernels may begin while the one in front on their stream runs, but not in front of an event that the stream waits for:
+    keys appended and queries made on a side stream that is late, eagerly and in a graph with a fork and a join."""
+    gen, dtype, page, heads, kv_heads, d = _gen(44), torch.bfloat16, 16, 8, 2, 64
+    cache = ftg.PagedCache.empty(1, 64, page, kv_heads, d, dtype)
+    slow = _randn(gen, (4096, 4096), dtype)
+    lengths = [300, 17, 500]
+    source = [_randn(gen, (sum(lengths), h, d), dtype) for h in (heads, kv_heads, kv_heads)]
+    q, out = torch.empty_like(source[0]), torch.empty_like(source[0])
+    pages, table = _paged(np.random.RandomState(44), lengths, page, spare=0)
+    slots = torch.tensor([int(table[b, i // page]) * page + i % page for b, n in enumerate(lengths) for i in range(n)], device="cuda")
+    offsets, table = _offsets(lengths), torch.from_numpy(table).cuda()
+    held, tree, prompt = torch.tensor(lengths, dtype=torch.int32, device="cuda"), ftg.TreeAttention(heads, cache), ftg.PromptAttention(heads, kv_heads, d, dtype=dtype)
+    packed, side, main = torch.empty_like(out), torch.cuda.Stream(), torch.cuda.Stream()
+
+    def calls():
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(8):
+                torch.mm(slow, slow)
+            cache.append(0, source[1], source[2], slots)
+            q.copy_(source[0])
+        out.zero_(), packed.zero_()  # a short kernel right in front, on this stream
+        torch.cuda.current_stream().wait_stream(side)
+        tree.run(q, 0, offsets, table, held, out)
+        prompt.run(q, source[1], source[2], packed, offsets)
+
+    def clear():
+        torch.cuda.synchronize()
+        q.fill_(math.nan), cache.k.fill_(math.nan), cache.v.fill_(math.nan)
+        torch.cuda.synchronize()
+
+    graph = None
+    for turn in range(6):
+        clear()
+        with torch.cuda.stream(main):
+            if turn < 3:
+                calls()
+            elif graph is None:
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, stream=main):
+                    calls()
+                graph.replay()
+            else:
+                graph.replay()
+        tree.report(), prompt.report()
+        at = 0
+        for n in lengths:
+            rows, visible = slice(at, at + n), torch.ones(n, n, dtype=torch.bool, device="cuda").tril()
+            for got in (out, packed):
+                _check_rows(got[rows], None, source[0][rows], source[1][rows], source[2][rows], visible, d ** -0.5)
+            at += n
+
+
 def test_page_operations_and_rotary_positions_in_graphs_and_on_streams(ftg):
     gen, dtype = _gen(33), torch.bfloat16
     cache = ftg.PagedCache.empty(2, 12, 8, 2, 64, dtype)
