@@ -122,8 +122,8 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 // The same on the FMA pipe: x = r + f with r a whole number (adding 1.5 * 2^23 rounds to it) and |f| <= 1/2; 2^f is the
-// polynomial of degree 5 with the smallest relative error there and a constant term of 1 (9.1e-8; fitted by least squares,
-// reweighted towards the largest errors until they level out), 2^r goes into the exponent bits.  At -127 and below the
+// polynomial of degree 5 with the smallest relative error there and a constant term of 1 (fitted by least squares, reweighted
+// towards the largest errors; with these constants 1.1e-7 in exact arithmetic, 1.7e-7 in 32 bits), 2^r goes into the exponent bits.  At -127 and below the
 // result is 0, and a NaN stays one.
 __device__ __forceinline__ float exp2_polynomial(float x) {
   float y;

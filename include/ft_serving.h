@@ -6,13 +6,15 @@
  * beside the protected attention of ft_attention.h and share its error codes and
  * ft_gemm_last_error().
  *
- * Common rules.  Element types are FT_SRC_BF16 and FT_SRC_F16 (ft_gemm.h); sums,
- * softmax statistics and angles are held in 32 bits or more and every result is
- * rounded once.  All pointers inside the structures are device pointers unless a
- * field says "host".  Calls are asynchronous on `stream`, allocate nothing, keep
- * nothing between calls and may be captured into a graph; two calls may run at the
- * same time on different streams when they write different memory (workspaces
- * included).  They run on the calling thread's current device.
+ * Common rules.  Element types are FT_SRC_BF16 and FT_SRC_F16 (ft_gemm.h); sums and
+ * softmax statistics are held in 32 bits, angles formed in 64, and every result is
+ * rounded once.  The attention also rounds each probability once, to the element type,
+ * as an operand of its second product (the denominator adds them up before that).
+ * All pointers inside the structures are device pointers unless a field says "host".
+ * Calls are asynchronous on `stream`, allocate nothing, keep nothing between calls and
+ * may be captured into a graph; two calls may run at the same time on different streams
+ * when they write different memory (workspaces included).  They run on the calling
+ * thread's current device.
  */
 #ifndef FT_SERVING_H
 #define FT_SERVING_H
@@ -40,8 +42,9 @@ typedef struct {
  *   (a, b) -> magnitude * (a cos - b sin, a sin + b cos)
  * with the pairs (i, i + rotary_dim/2), or (2i, 2i + 1) when interleaved; the
  * elements from rotary_dim on are copied.  f_i = base^(-2 i / rotary_dim), scaled for
- * long contexts by one of FT_ROTARY_*.  Angles are formed in 64 bits, so positions of
- * any size keep their accuracy. */
+ * long contexts by one of FT_ROTARY_*.  Frequencies are doubles, an angle is one product and
+ * one reduction in 64 bits: off by 2^-52 of its turns (p * f_i / 2pi), which after 2^24 of them
+ * (positions of 100 million) is still less than the rounding of its sine in 32 bits. */
 #define FT_ROTARY_PLAIN 0
 #define FT_ROTARY_LINEAR 1   /* f_i / factor */
 #define FT_ROTARY_BASE 2     /* base * factor^(rotary_dim / (rotary_dim - 2)) */
@@ -66,7 +69,8 @@ void ft_rotary_options_default(ft_rotary_options* options, int head_dim);
 /* The rotary_dim/2 frequencies in radians per position, into host memory. */
 int ft_rotary_frequencies(const ft_rotary_options* options, double* host_out);
 
-/* The handle holds the frequencies on the current device and is not written by runs. */
+/* The handle holds the frequencies on the current device and is not written by runs.  Captured graphs
+ * read it too: it is destroyed after them. */
 int ft_rotary_prepare(ft_rotary_handle** handle, const ft_rotary_options* options, void* stream);
 int ft_rotary_destroy(ft_rotary_handle* handle);
 
@@ -126,7 +130,8 @@ int ft_kv_cache_accept(const ft_kv_cache* cache, const int* page_table, int tabl
 /* ---- page pool (host) ------------------------------------------------------------
  * Which sequence holds which page.  A forked sequence shares its pages with its parent
  * until one of them writes: _extend then gives the writer a copy of the last, partly
- * filled page.  Calls that move contents return the pairs to hand to
+ * filled page.  (Places that both held when they were forked stay shared: they are written before
+ * the fork.)  Calls that move contents return the pairs to hand to
  * ft_kv_cache_copy_pages before the next append, and before _free or _truncate give a page
  * back that one of the pairs names.  One thread at a time. */
 typedef struct ft_page_pool ft_page_pool;
@@ -158,6 +163,9 @@ int ft_page_pool_compact(ft_page_pool* pool, int* host_sources, int* host_target
  * rows by 128 keys: counted with table_pages for each sequence over the cache, and with all of q and k
  * for a single packed sequence, and refused beyond; several packed sequences are counted on the device,
  * each with its own keys, and where they pass it the call writes FT_ERR_INVALID to `status` and no output.
+ *
+ * Values are added up in 32 bits by the tensor core, which cuts products off towards zero: over N
+ * keys by at most N 2^-27 of the sum, and never more than 2^-10.
  *
  * What lies behind a sequence's last key never reaches its output, whatever it is.  A key that some
  * rows of a sequence see and others do not has the probability zero in the others: K may hold
