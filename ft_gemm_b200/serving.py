@@ -351,8 +351,14 @@ class PagePool:
         return list(out[:self._value(self.lib.ft_page_pool_pages(self.handle, sequence, out, self.pages))])
 
     def _check_stream(self, stream: Optional[torch.cuda.Stream]):
-        if stream is not None and self.cache is not None:
-            _stream(self.cache.device, stream)  # refuses another device's, before anything changes
+        """Refuses what the copies could not be made on, before anything changes."""
+        if self.cache is None:
+            return
+        if stream is not None:
+            _stream(self.cache.device, stream)
+        with torch.cuda.stream(stream) if stream is not None else torch.cuda.device(self.cache.device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the page pool works on the host: a captured step leaves it out")
 
     def _move(self, pairs: List[Tuple[int, int]], stream: Optional[torch.cuda.Stream]):
         if pairs and self.cache is not None:

@@ -1045,6 +1045,30 @@ def test_a_call_waits_for_what_another_stream_has_written(ftg):
             at += n
 
 
+def test_the_pool_refuses_to_be_captured(ftg):
+    """Before anything changes: its copies would be lost, and the pages would be taken for copied."""
+    cache = ftg.PagedCache.empty(1, 6, 8, 1, 64)
+    cache.k.fill_(1.0), cache.v.fill_(1.0)
+    pool = ftg.PagePool(6, 8, cache)
+    first, a = pool.new_sequence(), pool.new_sequence()
+    pool.extend([first, a], [8, 5])
+    b = pool.fork(a)
+    pool.free(first)
+    before, x = [pool.page_list(s) for s in (a, b)], torch.zeros(4, device="cuda")
+    for call in (lambda: pool.extend([a], [1]), lambda: pool.compact()):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            x.add_(1.0)
+            with pytest.raises(RuntimeError, match="captured step"):
+                call()
+        graph.replay()
+        assert [pool.page_list(s) for s in (a, b)] == before and pool.length(a) == 5 and pool.free_pages() == 5
+    torch.cuda.synchronize()
+    assert x.tolist() == [2.0] * 4
+    side = torch.cuda.Stream()
+    assert pool.extend([a], [1], stream=side) == [(1, 0)] and pool.compact() == []  # otherwise as ever; the copy fills the hole
+
+
 def test_page_operations_and_rotary_positions_in_graphs_and_on_streams(ftg):
     gen, dtype = _gen(33), torch.bfloat16
     cache = ftg.PagedCache.empty(2, 12, 8, 2, 64, dtype)
