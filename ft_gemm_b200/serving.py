@@ -448,10 +448,12 @@ class _Attention:
 
     def report(self):
         """Waits for the device and raises if the output of an earlier run is not valid: a device-side wait gave up, or packed
-        prompts made more tiles than can be numbered."""
+        prompts made more tiles than can be numbered.  What was reported once does not count against later runs."""
         torch.cuda.synchronize(self.device)
         code = int(self.status.item())
         if code != _abi.FT_OK:
+            self.status.zero_()
+            torch.cuda.synchronize(self.device)  # before any stream runs a kernel that writes to it
             why = "an earlier run had too many tiles and wrote nothing" if code == _abi.FT_ERR_INVALID else (
                 "a device-side wait expired; the output of an earlier run is not valid")
             raise _abi.FtGemmError(code, why)

@@ -1069,6 +1069,19 @@ def test_the_pool_refuses_to_be_captured(ftg):
     assert pool.extend([a], [1], stream=side) == [(1, 0)] and pool.compact() == []  # otherwise as ever; the copy fills the hole
 
 
+@pytest.mark.parametrize("code", ["FT_ERR_TIMEOUT", "FT_ERR_INVALID"])
+def test_a_reported_failure_does_not_count_against_later_runs(ftg, code):
+    """The status word is set here as a kernel would set it."""
+    x, op = torch.ones((5, 2, 64), dtype=torch.bfloat16, device="cuda"), ftg.PromptAttention(2, 2, 64)
+    op.status.fill_(getattr(ftg, code))
+    with pytest.raises(ftg.FtGemmError, match="not valid" if code == "FT_ERR_TIMEOUT" else "wrote nothing"):
+        op.report()
+    out = torch.empty_like(x)
+    op.run(x, x, x, out, _offsets([5]))
+    op.report()
+    assert bool((out == 1.0).all())
+
+
 def test_page_operations_and_rotary_positions_in_graphs_and_on_streams(ftg):
     gen, dtype = _gen(33), torch.bfloat16
     cache = ftg.PagedCache.empty(2, 12, 8, 2, 64, dtype)
